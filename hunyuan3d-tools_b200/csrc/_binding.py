@@ -83,11 +83,18 @@ SIGNATURES = {
     "hy3d_add_quantize_rows": [c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p],
     "hy3d_add_layernorm_quantize": [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p, c_int,
                                     ctypes.c_float, c_void_p, c_void_p, c_void_p],
+    "hy3d_rmsnorm": [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int64, c_int64, c_void_p, c_int, ctypes.c_float,
+                     c_void_p, c_void_p, c_void_p, c_void_p],
+    "hy3d_dequantize_rows": [c_void_p, c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p],
+    "hy3d_rotary": [c_void_p, c_int, c_int, c_int64, c_int64, c_int, c_int, c_int, c_void_p, c_int, c_int64, c_int64, c_int64,
+                    c_int64, c_void_p, c_void_p, ctypes.c_float, c_int, c_void_p],
+    "hy3d_linear_w4": [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int64,
+                       c_int64, c_int64, c_int, c_void_p],
     "hy3d_version": [],
 }
 
 # The argument lists above belong to this ABI version of the library (hy3d_version()).
-ABI_VERSION = 205
+ABI_VERSION = 206
 
 
 def configure(lib: ctypes.CDLL) -> ctypes.CDLL:
@@ -236,6 +243,86 @@ class _Base:
                 gamma.data_ptr() if gamma is not None else None,
                 beta.data_ptr() if beta is not None else None, code, float(eps), 1 if silu else 0,
                 y.data_ptr(), None, self._stream(x)), "hy3d_groupnorm_nhwc")
+        return y
+
+    @staticmethod
+    def _rows(t: torch.Tensor, name: str):
+        """(rows, row pitch) of a tensor whose last dimension is dense and whose leading dimensions step evenly."""
+        K = t.shape[-1]
+        rows, pitch = 1, None
+        for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+            if size != 1:
+                if pitch is not None and stride != pitch * rows:
+                    return None
+                pitch = stride if pitch is None else pitch
+                rows *= size
+        if t.numel() and (t.stride(-1) != 1 and K != 1):
+            return None
+        pitch = K if pitch is None else pitch
+        return (rows, pitch) if pitch >= K and pitch % 8 == 0 else None
+
+    def rmsnorm(self, x, gamma, eps, add=None, codes=False, normalised=True):
+        """Root-mean-square norm over the last dimension of x (..., K), or of x + add: ``(sum | None, y | None, q | None,
+        scale | None)``, the 16-bit values with ``normalised``, int8 codes (M,K) and scales (M) with ``codes``.  Rows
+        may lie apart (a slice of a wider tensor); other strides are copied first."""
+        half = (torch.float16, torch.bfloat16)
+        for t, name in ((x, "x"), (add, "add")):
+            if t is None and name == "add":
+                continue
+            if not isinstance(t, torch.Tensor) or not t.is_cuda:
+                raise RuntimeError(f"rmsnorm: {name} must be a CUDA tensor (no CPU fallback)")
+            if t.dtype not in half or t.dtype != x.dtype or t.shape != x.shape or t.device != x.device or t.dim() < 1:
+                raise RuntimeError(f"rmsnorm: {name} must be fp16 or bf16, of one type, shape and device "
+                                   f"({tuple(t.shape)} of {t.dtype} on {t.device})")
+            self._no_gradient(t, f"rmsnorm: {name}")
+        K = x.shape[-1]
+        if K == 0 or K % 8 or K > 16384:
+            raise RuntimeError(f"rmsnorm: the normalised dimension is {K}, expected a multiple of 8 up to 16384")
+        if gamma is not None:
+            if gamma.numel() != K or gamma.device != x.device or gamma.dtype not in half + (torch.float32,):
+                raise RuntimeError(f"rmsnorm: weight must have {K} values of fp16, bf16 or fp32 on {x.device}")
+            gamma = gamma.detach().contiguous()
+            if gamma.data_ptr() % 16:
+                gamma = gamma.clone()
+        M = x.numel() // K
+
+        def rows(t):
+            at = self._rows(t, "x") if t.data_ptr() % 16 == 0 else None
+            return (t, at[1]) if at is not None else (t.contiguous() if not t.is_contiguous() else t.clone(), K)
+        x, ldx = rows(x)
+        add, ld_add = rows(add) if add is not None else (None, 0)
+        total = torch.empty(x.shape, dtype=x.dtype, device=x.device) if add is not None else None
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if normalised else None
+        q = torch.empty((M, K), dtype=torch.int8, device=x.device) if codes else None
+        s = torch.empty((M,), dtype=torch.float32, device=x.device) if codes else None
+
+        def ptr(t):
+            return t.data_ptr() if t is not None else None
+        with torch.cuda.device(x.device):
+            self._check(self._lib.hy3d_rmsnorm(
+                x.data_ptr(), ldx, ptr(add), ld_add, ptr(total), _DTYPE_CODE[x.dtype], M, K, ptr(gamma),
+                _DTYPE_CODE[gamma.dtype] if gamma is not None else F32, float(eps), ptr(y), ptr(q), ptr(s), self._stream(x)),
+                "hy3d_rmsnorm")
+        return total, y, q, s
+
+    @staticmethod
+    def _no_gradient(t, what):
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{what} requires a gradient, and none is recorded here: call under torch.no_grad() or detach it")
+
+    def dequantize_rows(self, q, scale, dtype):
+        """int8 codes (M,K) and scales (M) -> the (M,K) values they stand for, rounded to fp16 or bf16."""
+        self._req(q, "q", torch.int8, 2)
+        self._req(scale, "scale", torch.float32, 1)
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise RuntimeError(f"dequantize_rows: dtype is {dtype}, expected fp16 or bf16")
+        M, K = q.shape
+        if scale.shape[0] != M or scale.device != q.device:
+            raise RuntimeError(f"dequantize_rows: scale must have {M} entries on {q.device}")
+        y = torch.empty((M, K), dtype=dtype, device=q.device)
+        with torch.cuda.device(q.device):
+            self._check(self._lib.hy3d_dequantize_rows(q.data_ptr(), scale.data_ptr(), M, K, _DTYPE_CODE[dtype], y.data_ptr(),
+                                                       self._stream(q)), "hy3d_dequantize_rows")
         return y
 
     def quantizer_enum_check(self, dtype):
@@ -399,6 +486,39 @@ class TcGemmModule(_Base):
                 w_int8.data_ptr(), w_scale.data_ptr(), _DTYPE_CODE[w_scale.dtype], bptr, bcode,
                 out.data_ptr(), _DTYPE_CODE[x.dtype], M, N, K, epilogue, cta_group, block_n,
                 self._stream(x)), "hy3d_linear_w8a8_dense")
+        return out
+
+    def int4_linear(self, x, w, scale, zero, bias, epilogue=EPI_LINEAR):
+        """x (M,K) f16/bf16; w (N/16, K/64, 512) uint8, scale (N/16, K/group, 16) f16/bf16, zero likewise uint8 or None, as
+        ``Int4Linear`` lays them out; bias (N) or None -> (M,N), (M,N/2) with the GEGLU epilogue, in x's dtype."""
+        self._req(x, "x", (torch.float16, torch.bfloat16), 2)
+        self._req(w, "w", torch.uint8, 3)
+        self._req(scale, "scale", (torch.float16, torch.bfloat16), 3)
+        M, K = x.shape
+        N = 16 * w.shape[0]
+        if w.shape[1] * 64 != K or w.shape[2] != 512:
+            raise RuntimeError(f"K mismatch: x has {K}, the weight {64 * w.shape[1]}")
+        groups = scale.shape[1]
+        if scale.shape[0] != w.shape[0] or scale.shape[2] != 16 or groups < 1 or K % groups:
+            raise RuntimeError("scale must be (N/16, groups, 16) with a whole number of columns per group")
+        if zero is not None:
+            self._req(zero, "zero", torch.uint8, 3)
+            if zero.shape != scale.shape:
+                raise RuntimeError("zero must have the shape of scale")
+        bptr, bcode = self._opt_bias(bias)
+        if bptr is not None:
+            self._req(bias, "bias", (torch.float16, torch.bfloat16, torch.float32), 1)
+            if bias.shape[0] != N:
+                raise RuntimeError(f"bias must have {N} entries")
+        for t in (w, scale, zero, bias):
+            if t is not None and t.device != x.device:
+                raise RuntimeError(f"the layer is on {t.device}, its input on {x.device}")
+        out = torch.empty(self._out_shape(M, N, epilogue), dtype=x.dtype, device=x.device)
+        with torch.cuda.device(x.device):
+            self._check(self._lib.hy3d_linear_w4(
+                x.data_ptr(), _DTYPE_CODE[x.dtype], K, w.data_ptr(), scale.data_ptr(), _DTYPE_CODE[scale.dtype],
+                zero.data_ptr() if zero is not None else None, K // groups, bptr, bcode, out.data_ptr(), M, N, K, epilogue,
+                self._stream(x)), "hy3d_linear_w4")
         return out
 
     def int8_linear_tc_static(self, x, w_int8, w_scale, bias, out=None, epilogue=EPI_LINEAR):

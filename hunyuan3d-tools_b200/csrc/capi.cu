@@ -63,6 +63,8 @@ int check_device() {
 
 }  // namespace
 
+int device_ok() { return check_device(); }
+
 int device_sm_count() {
   int sms = 0, major = 0;
   return query_device(&sms, &major) == HY3D_OK ? sms : -1;
@@ -272,6 +274,29 @@ int hy3d_add_layernorm_quantize(const void* x, const void* add, void* sum, int x
   if (M > 0 && (!add || !sum)) return HY3D_ERR_ARG;
   return layernorm_quantize(x, add, x_dtype, M, K, K, gamma, beta, gb_dtype, eps, q, scale, sum,
                             static_cast<cudaStream_t>(stream));
+}
+
+int hy3d_rmsnorm(const void* x, int64_t ldx, const void* add, int64_t ld_add, void* sum, int x_dtype, int64_t M, int64_t K,
+                 const void* gamma, int g_dtype, float eps, void* y, int8_t* q, float* scale, void* stream) {
+  return rms::rmsnorm(x, ldx, add, ld_add, sum, x_dtype, M, K, gamma, g_dtype, eps, y, q, scale, static_cast<cudaStream_t>(stream));
+}
+
+int hy3d_dequantize_rows(const int8_t* q, const float* scale, int64_t M, int64_t K, int out_dtype, void* y, void* stream) {
+  return rms::dequantize_rows(q, scale, M, K, out_dtype, y, static_cast<cudaStream_t>(stream));
+}
+
+int hy3d_rotary(const hy3d_rotary_side* sides, int n_sides, int dtype, int64_t batch, int64_t n, int dim, int rot, int interleaved,
+                const void* positions, int positions_64, int64_t pb, int64_t pn, int64_t pa, int64_t offset,
+                const uint64_t* turns, const uint8_t* axis, float amplitude, int inverse, void* stream) {
+  return rotary::apply(sides, n_sides, dtype, batch, n, dim, rot, interleaved, positions, positions_64, pb, pn, pa, offset, turns,
+                       axis, amplitude, inverse, static_cast<cudaStream_t>(stream));
+}
+
+int hy3d_linear_w4(const void* x, int x_dtype, int64_t ldx, const void* w, const void* scale, int scale_dtype, const void* zero,
+                   int64_t group, const void* bias, int bias_dtype, void* out, int64_t M, int64_t N, int64_t K, int epilogue,
+                   void* stream) {
+  return w4::linear(x, x_dtype, ldx, w, scale, scale_dtype, zero, group, bias, bias_dtype, out, M, N, K, epilogue,
+                    static_cast<cudaStream_t>(stream));
 }
 
 int64_t hy3d_groupnorm_workspace_floats(int64_t B, int64_t HW, int groups) {

@@ -17,6 +17,7 @@
 #include <ATen/Context.h>
 #include <ATen/autocast_mode.h>
 #include <ATen/core/Tensor.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -49,6 +50,10 @@ struct Api {
   HY3D_FN(hy3d_add_quantize_rows);
   HY3D_FN(hy3d_add_layernorm_quantize);
   HY3D_FN(hy3d_quantize_weight);
+  HY3D_FN(hy3d_rmsnorm);
+  HY3D_FN(hy3d_dequantize_rows);
+  HY3D_FN(hy3d_rotary);
+  HY3D_FN(hy3d_linear_w4);
   HY3D_FN(hy3d_status_string);
 } api;
 #undef HY3D_FN
@@ -485,14 +490,14 @@ PyObject* quantize_weight(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // `forward`, any hook (of the instance or global), a compiled or traced call, and whatever the functions above
 // decline.
 struct Names {
-  PyObject *dict, *buffers, *parameters, *mode, *epilogue, *bias, *wq, *scale, *comp, *meta, *forward, *compiled, *weight,
+  PyObject *w4, *zero, *dict, *buffers, *parameters, *mode, *epilogue, *bias, *wq, *scale, *comp, *meta, *forward, *compiled, *weight,
       *eps, *fused, *silu, *groups, *shape, *dtype, *q, *act_scale, *conv_groups;
   PyObject* hooks[4];
 } names;
 struct Registered {
   PyTypeObject* type = nullptr;
   PyObject* forward = nullptr;
-} linear_class, layernorm_class, groupnorm_class;
+} linear_class, layernorm_class, groupnorm_class, int4_class, rmsnorm_classes[2];
 PyTypeObject* quantized_class = nullptr;
 PyObject* global_hooks[4] = {};
 
@@ -503,22 +508,23 @@ bool intern_names() {
       {&names.comp, "weight_sparse_comp"}, {&names.meta, "weight_sparse_meta"}, {&names.forward, "forward"},
       {&names.compiled, "_compiled_call_impl"}, {&names.weight, "weight"}, {&names.eps, "eps"}, {&names.fused, "fused"},
       {&names.silu, "silu"}, {&names.groups, "num_groups"}, {&names.shape, "shape"}, {&names.dtype, "dtype"},
-      {&names.q, "q"}, {&names.conv_groups, "groups"}, {&names.act_scale, "scale"}, {&names.hooks[0], "_backward_hooks"},
+      {&names.q, "q"}, {&names.w4, "weight_int4"}, {&names.zero, "weight_zero"}, {&names.conv_groups, "groups"}, {&names.act_scale, "scale"}, {&names.hooks[0], "_backward_hooks"},
       {&names.hooks[1], "_backward_pre_hooks"}, {&names.hooks[2], "_forward_hooks"}, {&names.hooks[3], "_forward_pre_hooks"}};
   for (auto& n : all)
     if (!(*n.at = PyUnicode_InternFromString(n.text))) return false;
   return true;
 }
 
-// register_modules((Int8Linear, Int8LayerNorm, GroupNormNHWC | None), QuantizedActivation, 4 global hook dicts):
+// register_modules((Int8Linear, Int8LayerNorm, GroupNormNHWC | None, Int4Linear, AddRMSNorm, Int8RMSNorm), QuantizedActivation,
+// 4 global hook dicts):
 // the classes with the `forward` they have now.
 PyObject* register_modules(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 3 || !PyTuple_Check(a[0]) || !PyType_Check(a[1]) || !PyTuple_Check(a[2]) || PyTuple_GET_SIZE(a[2]) != 4) {
     PyErr_SetString(PyExc_TypeError, "register_modules(classes, quantized class, hook dicts)");
     return nullptr;
   }
-  Registered* regs[] = {&linear_class, &layernorm_class, &groupnorm_class};
-  for (Py_ssize_t i = 0; i < 3 && i < PyTuple_GET_SIZE(a[0]); ++i) {
+  Registered* regs[] = {&linear_class, &layernorm_class, &groupnorm_class, &int4_class, &rmsnorm_classes[0], &rmsnorm_classes[1]};
+  for (Py_ssize_t i = 0; i < 6 && i < PyTuple_GET_SIZE(a[0]); ++i) {
     PyObject* c = PyTuple_GET_ITEM(a[0], i);
     if (c == Py_None) continue;
     PyObject* f = PyType_Check(c) ? PyObject_GetAttr(c, names.forward) : nullptr;
@@ -661,6 +667,286 @@ PyObject* norm_call(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!pair) { Py_XDECREF(sum); Py_DECREF(r); return nullptr; }
   PyTuple_SET_ITEM(pair, 0, sum);
   PyTuple_SET_ITEM(pair, 1, r);
+  return pair;
+  END_HANDLE_TH_ERRORS
+}
+
+// A tensor whose gradient a caller expects, and none of these functions records.
+bool wants_gradient(const at::Tensor& t) { return t.requires_grad() && c10::GradMode::is_enabled(); }
+
+// The 4-bit layer of instance dictionary `dict` on a tensor.
+PyObject* int4_of(PyObject* layer, PyObject* dict, PyObject* px) {
+  HANDLE_TH_ERRORS
+  PyObject* buffers = PyDict_GetItemWithError(dict, names.buffers);
+  if (!buffers || !PyDict_Check(buffers)) return none();
+  auto get = [&](PyObject* name) {
+    PyObject* v = PyDict_GetItemWithError(buffers, name);
+    return v ? v : PyDict_GetItemWithError(dict, name);
+  };
+  PyObject *pw = get(names.w4), *pscale = get(names.scale), *pzero = get(names.zero), *pbias = get(names.bias);
+  PyObject* pe = PyDict_GetItemWithError(dict, names.epilogue);
+  if (!pe) pe = _PyType_Lookup(Py_TYPE(layer), names.epilogue);
+  if (!pw || !pscale || !pzero || !pbias || !pe || !PyUnicode_Check(pe)) return none();
+  int epi = -1, i = 0;
+  for (const char* text : {"linear", "gelu", "geglu"}) {
+    if (PyUnicode_CompareWithASCIIString(pe, text) == 0) epi = i;
+    ++i;
+  }
+  const at::Tensor *x = plain(px), *w = plain(pw), *s = plain(pscale), *z = pzero == Py_None ? nullptr : plain(pzero);
+  if (epi < 0 || !x || !w || !s || (pzero != Py_None && !z) || x->dim() < 1 || w->dim() != 3 || s->dim() != 3 ||
+      w->scalar_type() != at::kByte || w->size(2) != 512 || s->size(2) != 16 || s->size(0) != w->size(0) || s->size(1) < 1 ||
+      w->device() != x->device() || s->device() != x->device())
+    return none();
+  if (z && (z->scalar_type() != at::kByte || z->sizes() != s->sizes() || z->device() != x->device())) return none();
+  const int code = half_code(x->scalar_type()), scale_code = half_code(s->scalar_type());
+  const int64_t N = 16 * w->size(0), K = 64 * w->size(1);
+  const int64_t M = K > 0 ? x->numel() / K : 0;
+  if (code < 0 || scale_code < 0 || M <= 0 || x->size(-1) != K || K % s->size(1) || wants_gradient(*x) ||
+      (reinterpret_cast<uintptr_t>(x->const_data_ptr()) & 15))
+    return none();
+  const void* bias = nullptr;
+  int bias_code = HY3D_F16;
+  if (pbias != Py_None) {
+    const at::Tensor* b = plain(pbias);
+    if (!b || b->dim() != 1 || b->size(0) != N || b->device() != x->device()) return none();
+    bias_code = param_code(b->scalar_type());
+    if (bias_code < 0) return none();
+    bias = b->const_data_ptr();
+  }
+  c10::cuda::CUDAGuard guard(x->device());
+  cudaStream_t st = c10::cuda::getCurrentCUDAStream(x->device().index()).stream();
+  at::Tensor y = out_like(x->sizes().slice(0, x->dim() - 1), epi == HY3D_EPI_GEGLU ? N / 2 : N, x->scalar_type(), x->device());
+  const int rc = api.hy3d_linear_w4(x->const_data_ptr(), code, K, w->const_data_ptr(), s->const_data_ptr(), scale_code,
+                                    z ? z->const_data_ptr() : nullptr, K / s->size(1), bias, bias_code, y.mutable_data_ptr(),
+                                    M, N, K, epi, st);
+  if (rc != HY3D_OK) return failed("hy3d_linear_w4", rc);
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+// int4_call(layer, x) -> y | None: calling an Int4Linear
+PyObject* int4_call(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  PyObject* dict = n == 2 ? plain_module(a[0], int4_class) : nullptr;
+  return dict ? int4_of(a[0], dict, a[1]) : none();
+}
+// int4_forward(layer, x) -> y | None: Int4Linear.forward, also of subclasses
+PyObject* int4_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 2) return none();
+  PyObject* dict = PyObject_GetAttr(a[0], names.dict);
+  if (!dict) return nullptr;
+  Py_DECREF(dict);
+  return PyDict_Check(dict) ? int4_of(a[0], dict, a[1]) : none();
+}
+
+// rms_call(layer, x, add | None) -> y | None, or (x + add, y) | None: calling an AddRMSNorm (y a tensor) or an
+// Int8RMSNorm (y a QuantizedActivation)
+PyObject* rms_call(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 3) return none();
+  const bool codes = Py_TYPE(a[0]) == rmsnorm_classes[1].type;
+  PyObject* dict = plain_module(a[0], rmsnorm_classes[codes]);
+  PyObject* params = dict ? PyDict_GetItemWithError(dict, names.parameters) : nullptr;
+  PyObject* eps = dict ? PyDict_GetItemWithError(dict, names.eps) : nullptr;
+  if (!params || !PyDict_Check(params) || !eps || !PyFloat_Check(eps)) return none();
+  PyObject* gamma = PyDict_GetItemWithError(params, names.weight);
+  const at::Tensor *x = plain(a[1]), *add = a[2] == Py_None ? nullptr : plain(a[2]);
+  if (!gamma || !x || x->dim() < 1 || wants_gradient(*x)) return none();
+  if (a[2] != Py_None && (!add || add->scalar_type() != x->scalar_type() || add->device() != x->device() ||
+                          add->sizes() != x->sizes() || wants_gradient(*add)))
+    return none();
+  const int code = half_code(x->scalar_type());
+  const int64_t K = x->size(-1), M = K > 0 ? x->numel() / K : 0;
+  if (code < 0 || M <= 0 || (K & 7) || K > 16384) return none();
+  const Affine f(gamma, Py_None, K, x->device());
+  uintptr_t at16 = reinterpret_cast<uintptr_t>(x->const_data_ptr()) | reinterpret_cast<uintptr_t>(f.gamma);
+  if (add) at16 |= reinterpret_cast<uintptr_t>(add->const_data_ptr());
+  if (!f.ok || (at16 & 15)) return none();
+  c10::cuda::CUDAGuard guard(x->device());
+  cudaStream_t st = c10::cuda::getCurrentCUDAStream(x->device().index()).stream();
+  at::Tensor sum, y, q, s;
+  if (add) sum = at::Tensor(at::detail::empty_cuda(x->sizes(), x->scalar_type(), x->device(), std::nullopt));
+  if (codes) {
+    q = at::Tensor(at::detail::empty_cuda({M, K}, at::kChar, x->device(), std::nullopt));
+    s = at::Tensor(at::detail::empty_cuda({M}, at::kFloat, x->device(), std::nullopt));
+  } else {
+    y = at::Tensor(at::detail::empty_cuda(x->sizes(), x->scalar_type(), x->device(), std::nullopt));
+  }
+  const int rc = api.hy3d_rmsnorm(x->const_data_ptr(), K, add ? add->const_data_ptr() : nullptr, K, add ? sum.mutable_data_ptr() : nullptr,
+                                  code, M, K, f.gamma, f.code, static_cast<float>(PyFloat_AS_DOUBLE(eps)),
+                                  codes ? nullptr : y.mutable_data_ptr(), codes ? q.mutable_data_ptr<int8_t>() : nullptr,
+                                  codes ? s.mutable_data_ptr<float>() : nullptr, st);
+  if (rc != HY3D_OK) return failed("hy3d_rmsnorm", rc);
+  PyObject* r = codes ? quantized_object(a[1], std::move(q), std::move(s)) : THPVariable_Wrap(std::move(y));
+  if (!add || !r) return r;
+  PyObject* total = THPVariable_Wrap(std::move(sum));
+  PyObject* pair = total ? PyTuple_New(2) : nullptr;
+  if (!pair) { Py_XDECREF(total); Py_DECREF(r); return nullptr; }
+  PyTuple_SET_ITEM(pair, 0, total);
+  PyTuple_SET_ITEM(pair, 1, r);
+  return pair;
+  END_HANDLE_TH_ERRORS
+}
+
+// dequantize(q (M,K), scale (M), dtype, shape) -> the values, of that shape | None
+PyObject* dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4 || !THPDtype_Check(a[2])) return none();
+  const at::Tensor *q = plain(a[0]), *s = plain(a[1]);
+  const at::ScalarType type = reinterpret_cast<THPDtype*>(a[2])->scalar_type;
+  if (!q || !s || half_code(type) < 0 || q->dim() != 2 || s->dim() != 1 || q->scalar_type() != at::kChar ||
+      s->scalar_type() != at::kFloat || s->device() != q->device() || s->size(0) != q->size(0))
+    return none();
+  const int64_t M = q->size(0), K = q->size(1);
+  c10::SmallVector<int64_t, 6> lead;
+  if (M <= 0 || K <= 0 || (K & 7) || (reinterpret_cast<uintptr_t>(q->const_data_ptr()) & 7) || !lead_shape(a[3], M, K, &lead)) return none();
+  c10::cuda::CUDAGuard guard(q->device());
+  cudaStream_t st = c10::cuda::getCurrentCUDAStream(q->device().index()).stream();
+  at::Tensor y = out_like(lead, K, type, q->device());
+  const int rc = api.hy3d_dequantize_rows(q->const_data_ptr<int8_t>(), s->const_data_ptr<float>(), M, K, half_code(type),
+                                          y.mutable_data_ptr(), st);
+  if (rc != HY3D_OK) return failed("hy3d_dequantize_rows", rc);
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// Queries or keys of a rotary call: batch, tokens and heads with their strides.
+struct Turned {
+  const at::Tensor* t = nullptr;
+  int64_t b = 1, n = 0, h = 0, sb = 0, sn = 0, sh = 0;
+  Turned(PyObject* o, int64_t dim) {
+    if (!THPVariable_CheckExact(o)) return;
+    const at::Tensor& v = THPVariable_Unpack(o);
+    const int64_t d = v.dim();
+    if (!v.is_cuda() || v.layout() != at::kStrided || (d != 3 && d != 4) || half_code(v.scalar_type()) < 0 || v.size(-1) != dim ||
+        (v.stride(-1) != 1 && dim > 1) || wants_gradient(v))
+      return;
+    n = v.size(d - 3); h = v.size(d - 2); sn = v.stride(d - 3); sh = v.stride(d - 2);
+    if (d == 4) { b = v.size(0); sb = v.stride(0); }
+    t = &v;
+  }
+  int64_t row(int64_t dim) const { return (h - 1) * sh + dim; }                  // elements from a token's first to its last
+  int64_t sequence(int64_t dim) const { return (n - 1) * sn + row(dim); }
+  // Whether no two elements lie in the same place: each stride steps over all that the smaller ones reach.
+  bool separate(int64_t dim) const {
+    int64_t size[3] = {b, n, h}, stride[3] = {sb, sn, sh};
+    for (int i = 0; i < 3; ++i)
+      for (int j = i + 1; j < 3; ++j)
+        if (stride[j] < stride[i]) { std::swap(stride[i], stride[j]); std::swap(size[i], size[j]); }
+    int64_t reach = dim;
+    for (int i = 0; i < 3; ++i) {
+      if (size[i] <= 1) continue;
+      if (stride[i] < reach) return false;
+      reach += (size[i] - 1) * stride[i];
+    }
+    return true;
+  }
+};
+// Whether two tensors that are turned in place share no element: apart altogether, or side by side in every sequence or
+// in every token of equal steps (a stacked projection).
+bool apart(const Turned& a, const Turned& b, int64_t dim) {
+  if (a.t->numel() == 0 || b.t->numel() == 0) return true;
+  const int64_t size = a.t->element_size();
+  const char *pa = static_cast<const char*>(a.t->const_data_ptr()), *pb = static_cast<const char*>(b.t->const_data_ptr());
+  const int64_t gap = (pb - pa) / size;
+  auto beside = [&](int64_t ea, int64_t eb, int64_t step) {       // intervals of ea and eb elements, repeated every `step`
+    return gap >= 0 ? gap >= ea && gap + eb <= step : -gap >= eb && -gap + ea <= step;
+  };
+  constexpr int64_t kNever = int64_t{1} << 62;
+  const int64_t whole_a = (a.b - 1) * a.sb + a.sequence(dim), whole_b = (b.b - 1) * b.sb + b.sequence(dim);
+  if (beside(whole_a, whole_b, kNever)) return true;
+  if (a.sb == b.sb && a.sb > 0 && beside(a.sequence(dim), b.sequence(dim), a.sb)) return true;
+  const bool batches_apart = a.b == 1 || (a.sb == b.sb && a.sb >= (a.n - 1) * a.sn + a.sn && a.sn == b.sn);
+  return a.sn == b.sn && a.sn > 0 && batches_apart && beside(a.row(dim), b.row(dim), a.sn);
+}
+
+// rotary(plan, q, k | None, positions | None, offset, inverse, inplace) -> q | (q, k) | None; `plan` is RotaryPositions' own:
+// (head dimensions, rotated ones, axes, interleaved, turns, axis of each pair, amplitude)
+PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t argc) {
+  HANDLE_TH_ERRORS
+  if (argc != 7 || !PyTuple_CheckExact(a[0]) || PyTuple_GET_SIZE(a[0]) != 7) return none();
+  PyObject* const* plan = &PyTuple_GET_ITEM(a[0], 0);
+  long dim = 0, rot = 0, axes = 0;
+  if (!small_int(plan[0], 1, 1 << 24, &dim) || !small_int(plan[1], 2, 512, &rot) || !small_int(plan[2], 1, 255, &axes) ||
+      !PyBytes_CheckExact(plan[4]) || PyBytes_GET_SIZE(plan[4]) != 4 * rot || !PyBytes_CheckExact(plan[5]) ||
+      PyBytes_GET_SIZE(plan[5]) != rot / 2 || !PyFloat_CheckExact(plan[6]) || !PyLong_CheckExact(a[4]) || !PyBool_Check(a[5]) ||
+      !PyBool_Check(a[6]))
+    return none();
+  int overflow = 0;
+  const int64_t offset = PyLong_AsLongLongAndOverflow(a[4], &overflow);
+  if (overflow) return none();
+  const bool both = a[2] != Py_None, inplace = a[6] == Py_True;
+  const Turned side[2] = {Turned(a[1], dim), Turned(both ? a[2] : a[1], dim)};
+  const int sides = both ? 2 : 1;
+  for (int i = 0; i < sides; ++i)
+    if (!side[i].t || side[i].t->dim() != side[0].t->dim() || side[i].t->scalar_type() != side[0].t->scalar_type() ||
+        side[i].t->device() != side[0].t->device() || side[i].b != side[0].b || side[i].n != side[0].n ||
+        (inplace && !side[i].separate(dim)))
+      return none();
+  if (inplace && both && !apart(side[0], side[1], dim)) return none();
+  const at::Tensor& q = *side[0].t;
+  const int64_t b = side[0].b, n = side[0].n;
+  const void* positions = nullptr;
+  bool wide = false;
+  int64_t pb = 0, pn = 0, pa = 0;
+  if (a[3] != Py_None) {
+    if (!THPVariable_CheckExact(a[3]) || offset) return none();
+    const at::Tensor& p = THPVariable_Unpack(a[3]);
+    wide = p.scalar_type() == at::kLong;
+    if (p.device() != q.device() || p.layout() != at::kStrided || (!wide && p.scalar_type() != at::kInt)) return none();
+    // (tokens) or (batch, tokens), the axes behind; a single axis may leave its dimension out
+    for (int batched = 0; batched < (q.dim() == 4 ? 2 : 1) && !positions; ++batched)
+      for (int with_axes = axes == 1 ? 0 : 1; with_axes < 2 && !positions; ++with_axes) {
+        if (p.dim() != 1 + batched + with_axes || p.size(batched) != n || (batched && p.size(0) != b) ||
+            (with_axes && p.size(batched + 1) != axes))
+          continue;
+        positions = p.const_data_ptr();
+        pb = batched ? p.stride(0) : 0;
+        pn = p.stride(batched);
+        pa = with_axes ? p.stride(batched + 1) : 0;
+        if (p.numel() == 0) positions = &p;       // nothing is read
+      }
+    if (!positions) return none();
+  } else if (axes != 1) {
+    return none();
+  }
+  c10::cuda::CUDAGuard guard(q.device());
+  cudaStream_t st = c10::cuda::getCurrentCUDAStream(q.device().index()).stream();
+  at::Tensor out[2];
+  hy3d_rotary_side s[2];
+  for (int i = 0; i < sides; ++i) {
+    const Turned& t = side[i];
+    if (t.h > 1 << 20) return none();
+    s[i].src = t.t->const_data_ptr();
+    s[i].src_b = t.sb; s[i].src_n = t.sn; s[i].src_h = t.sh;
+    s[i].heads = static_cast<int>(t.h);
+    if (inplace) {
+      out[i] = *t.t;
+      out[i].unsafeGetTensorImpl()->bump_version();
+      s[i].dst_b = t.sb; s[i].dst_n = t.sn; s[i].dst_h = t.sh;
+    } else {
+      out[i] = at::Tensor(at::detail::empty_cuda(t.t->sizes(), t.t->scalar_type(), t.t->device(), std::nullopt));
+      s[i].dst_h = dim; s[i].dst_n = t.h * dim; s[i].dst_b = n * t.h * dim;
+    }
+    s[i].dst = out[i].mutable_data_ptr();
+  }
+  const int rc = api.hy3d_rotary(s, sides, half_code(q.scalar_type()), b, n, static_cast<int>(dim), static_cast<int>(rot),
+                                 plan[3] == Py_True, positions, wide, pb, pn, pa, offset,
+                                 reinterpret_cast<const uint64_t*>(PyBytes_AS_STRING(plan[4])),
+                                 reinterpret_cast<const uint8_t*>(PyBytes_AS_STRING(plan[5])),
+                                 static_cast<float>(PyFloat_AS_DOUBLE(plan[6])), a[5] == Py_True, st);
+  if (rc != HY3D_OK) return failed("hy3d_rotary", rc);
+  PyObject* r[2] = {nullptr, nullptr};
+  for (int i = 0; i < sides; ++i) {
+    if (inplace) { r[i] = a[1 + i]; Py_INCREF(r[i]); }
+    else r[i] = THPVariable_Wrap(std::move(out[i]));
+  }
+  if (!both || !r[0] || !r[1]) {
+    if (both) { Py_XDECREF(r[0]); Py_XDECREF(r[1]); return nullptr; }
+    return r[0];
+  }
+  PyObject* pair = PyTuple_New(2);
+  if (!pair) { Py_DECREF(r[0]); Py_DECREF(r[1]); return nullptr; }
+  PyTuple_SET_ITEM(pair, 0, r[0]);
+  PyTuple_SET_ITEM(pair, 1, r[1]);
   return pair;
   END_HANDLE_TH_ERRORS
 }
@@ -841,6 +1127,10 @@ PyObject* open_library(PyObject*, PyObject* arg) {
   HY3D_SYM(hy3d_add_quantize_rows);
   HY3D_SYM(hy3d_add_layernorm_quantize);
   HY3D_SYM(hy3d_quantize_weight);
+  HY3D_SYM(hy3d_rmsnorm);
+  HY3D_SYM(hy3d_dequantize_rows);
+  HY3D_SYM(hy3d_rotary);
+  HY3D_SYM(hy3d_linear_w4);
   HY3D_SYM(hy3d_status_string);
 #undef HY3D_SYM
   Py_RETURN_NONE;
@@ -854,6 +1144,11 @@ PyMethodDef methods[] = {
     HY3D_FAST(layer_forward),
     HY3D_FAST(norm_call),
     HY3D_FAST(groupnorm_call),
+    HY3D_FAST(int4_call),
+    HY3D_FAST(int4_forward),
+    HY3D_FAST(rms_call),
+    HY3D_FAST(dequantize),
+    HY3D_FAST(rotary),
     HY3D_FAST(add_quantize),
     HY3D_FAST(add_bias),
     HY3D_FAST(concat_nhwc),

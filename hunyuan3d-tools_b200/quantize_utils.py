@@ -105,7 +105,7 @@ def _load_native():
             native = load_native()
             mod = nn.modules.module
             native.register_modules(
-                (Int8Linear, Int8LayerNorm, GroupNormNHWC), QuantizedActivation,
+                (Int8Linear, Int8LayerNorm, GroupNormNHWC, Int4Linear, AddRMSNorm, Int8RMSNorm), QuantizedActivation,
                 (mod._global_backward_hooks, mod._global_backward_pre_hooks, mod._global_forward_hooks,
                  mod._global_forward_pre_hooks))
             _NATIVE = native
@@ -157,6 +157,14 @@ class QuantizedActivation:
 
     reshape = view
 
+    def dequantize(self) -> torch.Tensor:
+        """The values that the codes stand for, rounded to the activation's type."""
+        y = (_NATIVE or _load_native()).dequantize(self.q, self.scale, self.dtype, self.shape)
+        if y is None:
+            from .csrc.build import load_int8_kernels
+            y = load_int8_kernels().dequantize_rows(self.q, self.scale, self.dtype).reshape(self.shape)
+        return y
+
 
 class Int8LayerNorm(nn.Module):
     """``nn.LayerNorm`` over the last dimension whose output is emitted as int8 codes plus
@@ -201,6 +209,59 @@ class Int8LayerNorm(nn.Module):
 
     def extra_repr(self) -> str:
         return f"{self.normalized_shape}, eps={self.eps}, output=int8 codes + per-token scales"
+
+
+class AddRMSNorm(nn.Module):
+    """``nn.RMSNorm`` over the last dimension, optionally of ``x + add``, in one kernel: ``norm(x)`` returns the normalised
+    activations, ``norm(x, add)`` returns ``(x + add, normalised)``, both in x's type -- a pre-norm block's residual stream
+    and the input of its next layer.  The sum is rounded before it is normalised, as a separate addition would have left
+    it.  Shares the parameter of the norm that it is made from (its 16-bit or fp32 weight, or none).  CUDA fp16 / bf16
+    inputs of up to 16384 dimensions (a multiple of 8); no gradient is recorded."""
+
+    _codes = False
+
+    def __init__(self, norm: nn.RMSNorm):
+        super().__init__()
+        if len(norm.normalized_shape) != 1:
+            raise RuntimeError(f"{type(self).__name__} normalises the last dimension only")
+        self.normalized_shape = tuple(norm.normalized_shape)
+        self.eps = norm.eps
+        self.weight = norm.weight
+        self._ik = None
+
+    def __call__(self, x, add=None):
+        # The direct way to the kernel where no hook, subclass or tracer stands in it.
+        if _NATIVE is not None:
+            y = _NATIVE.rms_call(self, x, add)
+            if y is not None:
+                return y
+        return super().__call__(x) if add is None else super().__call__(x, add)
+
+    def forward(self, x: torch.Tensor, add: torch.Tensor | None = None):
+        if self._ik is None:
+            _load_native()
+            from .csrc.build import load_int8_kernels
+            self._ik = load_int8_kernels()
+        if isinstance(x, torch.Tensor) and tuple(x.shape[-1:]) != self.normalized_shape:
+            raise RuntimeError(f"{type(self).__name__} normalises {self.normalized_shape[0]} dimensions, got {tuple(x.shape)}")
+        eps = self.eps
+        if eps is None:         # nn.RMSNorm's default
+            eps = torch.finfo(x.dtype).eps if isinstance(x, torch.Tensor) and x.is_floating_point() else 0.0
+        total, y, q, s = self._ik.rmsnorm(x, self.weight, eps, add, codes=self._codes, normalised=not self._codes)
+        if self._codes:
+            y = QuantizedActivation(q, s, x.shape, x.dtype)
+        return y if add is None else (total, y)
+
+    def extra_repr(self) -> str:
+        return f"{self.normalized_shape}, eps={self.eps}, output={'int8 codes + per-token scales' if self._codes else '16-bit'}"
+
+
+class Int8RMSNorm(AddRMSNorm):
+    """``AddRMSNorm`` whose normalised output is emitted as int8 codes plus per-token scales (``QuantizedActivation``),
+    the codes that its consumers, ``Int8Linear`` layers all of them, would have computed from the 16-bit output:
+    ``norm(x)`` returns it, ``norm(x, add)`` returns ``(x + add, it)``."""
+
+    _codes = True
 
 
 # ---------------------------------------------------------------------------------------
@@ -519,6 +580,261 @@ class Int8Linear(nn.Module):
 
 
 # ---------------------------------------------------------------------------------------
+#  Int4Linear
+# ---------------------------------------------------------------------------------------
+# Columns of a packed word's nibbles, lowest first: (word >> 4j) & 0x000F000F are columns 2j and 2j + 1.
+_NIBBLE_COLUMNS = (0, 2, 4, 6, 1, 3, 5, 7)
+
+
+def _pack_codes(codes: torch.Tensor) -> torch.Tensor:
+    """Codes (N,K) of 0..15 -> (N/16, K/64, 512) bytes in the order of csrc/linear_w4.cu."""
+    n, k = codes.shape
+    c = codes.to(torch.uint8).view(n // 16, 2, 8, k // 64, 2, 4, 8)          # row block, half, g, tile, sub, t, column
+    c = c.permute(0, 3, 2, 5, 4, 1, 6)[..., list(_NIBBLE_COLUMNS)]           # row block, tile, g, t, sub, half, nibble
+    return (c[..., 0::2] | c[..., 1::2] << 4).reshape(n // 16, k // 64, 512)
+
+
+def _unpack_codes(packed: torch.Tensor) -> torch.Tensor:
+    blocks, tiles, _ = packed.shape
+    p = packed.view(blocks, tiles, 8, 4, 2, 2, 4)
+    c = torch.stack([p & 15, p >> 4], dim=-1).flatten(-2)
+    inverse = [_NIBBLE_COLUMNS.index(i) for i in range(8)]
+    return c[..., inverse].permute(0, 5, 2, 1, 4, 3, 6).reshape(blocks * 16, tiles * 64)
+
+
+def _pack_groups(v: torch.Tensor) -> torch.Tensor:
+    """Per-group values (N, groups) -> (N/16, groups, 16) with rows g and g + 8 of a block side by side."""
+    n, groups = v.shape
+    return v.view(n // 16, 2, 8, groups).permute(0, 3, 2, 1).reshape(n // 16, groups, 16)
+
+
+def _unpack_groups(v: torch.Tensor) -> torch.Tensor:
+    blocks, groups, _ = v.shape
+    return v.view(blocks, groups, 8, 2).permute(0, 3, 2, 1).reshape(blocks * 16, groups)
+
+
+class Int4Linear(nn.Module):
+    """``nn.Linear`` with 4-bit weights and group scales, for layers that see few rows at a time: the weights are read at a
+    quarter of their 16-bit size, the activations stay in 16 bits::
+
+        W[n,k] = scale[n, k // group] * (code[n,k] - zero[n, k // group]),   zero = 8 where there are no zero points
+
+    Products are exact and sums fp32, the scale multiplies a group's sum, and the output is rounded once.  Stands beside
+    ``Int8Linear`` (same epilogues, ``concat``, ``interleave_geglu_rows``, checkpoints); the reference has no counterpart.
+    Any number of rows; in_features % 64 == 0, out_features % 16 == 0, groups of 32 or of a multiple of 64 columns that
+    divides in_features.  CUDA fp16 / bf16 only; no gradient is recorded.
+
+    Buffers: ``weight_int4`` (N/16, K/64, 512) uint8, ``weight_scale`` (N/16, groups, 16), ``weight_zero`` likewise uint8 or
+    None, in the kernel's order; ``codes()``, ``scales()`` and ``zeros()`` give them row by row."""
+
+    epilogue: str = "linear"
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, dtype: torch.dtype = torch.float16,
+                 group_size: int = 64, symmetric: bool = True):
+        super().__init__()
+        if in_features <= 0 or out_features <= 0 or in_features % 64 or out_features % 16:
+            raise RuntimeError("Int4Linear needs in_features % 64 == 0 and out_features % 16 == 0, "
+                               f"got {in_features} and {out_features}")
+        if group_size < 32 or (group_size != 32 and group_size % 64) or in_features % group_size:
+            raise RuntimeError("Int4Linear needs groups of 32 or of a multiple of 64 columns that divides in_features, "
+                               f"got {group_size} of {in_features}")
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise RuntimeError(f"Int4Linear keeps its scales in fp16 or bf16, got {dtype}")
+        self.in_features, self.out_features = in_features, out_features
+        blocks, groups = out_features // 16, in_features // group_size
+        self.register_buffer("weight_int4", torch.full((blocks, in_features // 64, 512), 0x88, dtype=torch.uint8))
+        self.register_buffer("weight_scale", torch.ones(blocks, groups, 16, dtype=dtype))
+        self.register_buffer("weight_zero", None if symmetric else torch.full((blocks, groups, 16), 8, dtype=torch.uint8))
+        self.register_buffer("bias", torch.zeros(out_features, dtype=dtype) if bias else None)
+
+    @property
+    def group_size(self) -> int:
+        return self.in_features // self.weight_scale.shape[1]
+
+    # -- construction ------------------------------------------------------------------
+    @staticmethod
+    @torch.no_grad()
+    def from_codes(codes, scale, zero=None, bias=None) -> "Int4Linear":
+        """From codes (N,K) of 0..15, scales (N, K/group) in fp16 or bf16 and zero points of the same shape (whole numbers
+        0..15; 8 without them), as other quantisers produce them; bias (N) or None."""
+        if codes.dim() != 2 or codes.is_floating_point() or scale.dim() != 2 or scale.shape[0] != codes.shape[0] \
+                or scale.shape[1] < 1 or codes.shape[1] % scale.shape[1]:
+            raise RuntimeError("Int4Linear.from_codes takes whole codes (N, K) and scales (N, K / group), "
+                               f"got {tuple(codes.shape)} of {codes.dtype} and {tuple(scale.shape)}")
+        if zero is not None and (zero.shape != scale.shape or zero.is_floating_point()):
+            raise RuntimeError("Int4Linear.from_codes takes whole zero points in the shape of the scales")
+        for name, t in (("codes", codes), ("zero", zero)):
+            if t is not None and t.numel() and (int(t.min()) < 0 or int(t.max()) > 15):
+                raise RuntimeError(f"Int4Linear.from_codes: {name} must lie between 0 and 15")
+        n, k = codes.shape
+        if bias is not None and tuple(bias.shape) != (n,):
+            raise RuntimeError(f"Int4Linear.from_codes: bias must have {n} entries, got {tuple(bias.shape)}")
+        with torch.device("meta"):      # the shape rules, without buffers that are replaced below
+            layer = Int4Linear(k, n, bias=False, dtype=scale.dtype, group_size=k // scale.shape[1])
+        layer.weight_int4 = _pack_codes(codes)
+        layer.weight_scale = _pack_groups(scale)
+        if zero is not None:
+            layer.weight_zero = _pack_groups(zero.to(torch.uint8))
+        if bias is not None:
+            layer.bias = bias.detach().to(scale.dtype).contiguous()
+        return layer
+
+    @staticmethod
+    @torch.no_grad()
+    def from_linear(linear: nn.Linear, group_size: int = 64, symmetric: bool = True) -> "Int4Linear":
+        """Round-to-nearest quantisation of an ``nn.Linear``, group by group, with the scale as it is stored:
+        symmetric ``scale = max|w| / 7``, codes ``round(w / scale) + 8``; otherwise ``scale = (max - min) / 15``, the range
+        widened to hold 0, and a zero point ``round(-min / scale)``."""
+        n, k = linear.weight.shape
+        dt = _param_dtype(linear)
+        with torch.device("meta"):
+            Int4Linear(k, n, bias=False, dtype=dt, group_size=group_size)
+        w = linear.weight.detach().float().view(n, k // group_size, group_size)
+        if symmetric:
+            scale, zero = w.abs().amax(-1) / 7, None
+        else:
+            low, high = w.amin(-1).clamp(max=0), w.amax(-1).clamp(min=0)
+            scale = (high - low) / 15
+        # not below the type's smallest normal number, where the quotients would lose their meaning
+        scale = scale.clamp(min=torch.finfo(dt).tiny).to(dt)
+        s = scale.float()[..., None]
+        if not symmetric:
+            zero = (-low / s[..., 0]).round().clamp(0, 15)
+        codes = ((w / s).round() + (8 if symmetric else zero[..., None])).clamp(0, 15).to(torch.uint8).view(n, k)
+        bias = None if linear.bias is None else linear.bias.detach()
+        return Int4Linear.from_codes(codes, scale, None if symmetric else zero.to(torch.uint8), bias)
+
+    @staticmethod
+    def concat(layers) -> "Int4Linear":
+        """One layer computing ``[l0(x) | l1(x) | ...]``; every output column keeps its bits."""
+        layers = list(layers)
+        first = layers[0]
+        for l in layers:
+            if not isinstance(l, Int4Linear):
+                raise TypeError("Int4Linear.concat takes Int4Linear layers")
+            if (l.in_features != first.in_features or l.epilogue != "linear" or (l.bias is None) != (first.bias is None)
+                    or l.weight_scale.shape[1] != first.weight_scale.shape[1] or l.weight_scale.dtype != first.weight_scale.dtype
+                    or (l.weight_zero is None) != (first.weight_zero is None)):
+                raise RuntimeError("Int4Linear.concat needs layers of the same in_features, group size, dtype, zero points and "
+                                   "bias presence with the plain linear epilogue")
+        with torch.device("meta"):
+            out = Int4Linear(first.in_features, sum(l.out_features for l in layers), bias=False, dtype=first.weight_scale.dtype,
+                             group_size=first.group_size)
+        for name in ("weight_int4", "weight_scale", "weight_zero", "bias"):
+            if getattr(first, name) is not None:
+                setattr(out, name, torch.cat([getattr(l, name) for l in layers]))
+        return out
+
+    @staticmethod
+    def concat_state(state_dict, prefix, parts):
+        """``Int8Linear.concat_state`` for 4-bit layers."""
+        names = ("weight_int4", "weight_scale", "weight_zero", "bias")
+        have = [[n for n in names if part + n in state_dict] for part in parts]
+        extra = [state_dict.get(part + "_extra_state") for part in parts]
+        if prefix + "weight_int4" in state_dict or not all("weight_int4" in h and h == have[0] for h in have) \
+                or any(e != extra[0] for e in extra):
+            return
+        for n in have[0]:
+            state_dict[prefix + n] = torch.cat([state_dict.pop(part + n) for part in parts])
+        for part in parts:
+            state_dict.pop(part + "_extra_state", None)
+        if extra[0] is not None:
+            state_dict[prefix + "_extra_state"] = extra[0]
+
+    def interleave_geglu_rows(self) -> "Int4Linear":
+        """Re-orders a GEGLU up-projection ([value(H) | gate(H)] output rows) into blocks of 16 value rows followed by their
+        16 gate rows and switches the layer to the fused ``value * gelu(gate)`` epilogue; it then returns H columns."""
+        if self.epilogue != "linear":
+            raise RuntimeError("the layer already has a fused epilogue")
+        if self.out_features % 32:
+            raise RuntimeError("GEGLU fusion needs out_features % 32 == 0")
+        half = self.out_features // 32          # blocks of 16 rows, as they are stored
+        idx = torch.arange(half, device=self.weight_scale.device)
+        blocks = torch.stack([idx, idx + half], dim=1).reshape(-1)
+        for name in ("weight_int4", "weight_scale", "weight_zero"):
+            if getattr(self, name) is not None:
+                setattr(self, name, getattr(self, name)[blocks].contiguous())
+        if self.bias is not None:
+            self.bias = self.bias.view(2 * half, 16)[blocks].reshape(-1)
+        self.epilogue = "geglu"
+        return self
+
+    # -- what is stored, row by row ------------------------------------------------------
+    def codes(self) -> torch.Tensor:
+        return _unpack_codes(self.weight_int4)
+
+    def scales(self) -> torch.Tensor:
+        return _unpack_groups(self.weight_scale)
+
+    def zeros(self) -> torch.Tensor | None:
+        return None if self.weight_zero is None else _unpack_groups(self.weight_zero)
+
+    def dequantize_weight(self) -> torch.Tensor:
+        """(N,K) fp32, rows in the stored order."""
+        c, z = self.codes().float(), self.zeros()
+        z = 8.0 if z is None else z.float().repeat_interleave(self.group_size, dim=1)
+        return (c - z) * self.scales().float().repeat_interleave(self.group_size, dim=1)
+
+    # -- checkpointing -----------------------------------------------------------------
+    def get_extra_state(self):
+        return {"epilogue": self.epilogue, "layout": "hy3d-int4-v1"}
+
+    def set_extra_state(self, state):
+        if state.get("layout") != "hy3d-int4-v1":
+            raise RuntimeError(f"unknown Int4Linear layout {state.get('layout')!r}")
+        self.epilogue = state.get("epilogue", "linear")
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        # Group size, zero points, bias and type are the checkpoint's.
+        src = state_dict.get(prefix + "weight_int4")
+        if src is not None and tuple(src.shape) == tuple(self.weight_int4.shape):
+            for name in ("weight_scale", "weight_zero", "bias"):
+                src, cur = state_dict.get(prefix + name), getattr(self, name)
+                if src is None:
+                    self.register_buffer(name, None if name != "weight_scale" else cur)
+                elif cur is None or cur.shape != src.shape or cur.dtype != src.dtype:
+                    self.register_buffer(name, torch.empty(src.shape, dtype=src.dtype, device=self.weight_int4.device))
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+
+    # -- forward ------------------------------------------------------------------------
+    def __call__(self, *args, **kwargs):
+        # The direct way to the kernel where no hook, subclass or tracer stands in it.
+        if _NATIVE is not None and len(args) == 1 and not kwargs:
+            y = _NATIVE.int4_call(self, args[0])
+            if y is not None:
+                return y
+        return super().__call__(*args, **kwargs)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        y = (_NATIVE or _load_native()).int4_forward(self, x)
+        if y is not None:
+            return y
+        if isinstance(x, QuantizedActivation):
+            raise RuntimeError("Int4Linear takes 16-bit activations, not int8 codes")
+        if not x.is_cuda:
+            raise RuntimeError("Int4Linear runs on CUDA tensors only (no CPU fallback)")
+        if x.dtype not in (torch.float16, torch.bfloat16):
+            raise RuntimeError(f"Int4Linear expects fp16 or bf16 activations, got {x.dtype}")
+        if x.dim() < 1 or x.shape[-1] != self.in_features:
+            raise RuntimeError(f"Int4Linear expects {self.in_features} input features, got {tuple(x.shape)}")
+        if self.epilogue not in _EPILOGUES:
+            raise RuntimeError(f"unknown Int4Linear.epilogue {self.epilogue!r}")
+        tc = _load_tc()
+        tc._no_gradient(x, "Int4Linear: the input")
+        x2 = x.detach().reshape(-1, self.in_features)
+        if not x2.is_contiguous():
+            x2 = x2.contiguous()
+        if x2.data_ptr() % 16:
+            x2 = x2.clone()
+        y = tc.int4_linear(x2, self.weight_int4, self.weight_scale, self.weight_zero, self.bias, _EPILOGUES[self.epilogue])
+        return y.reshape(*x.shape[:-1], y.shape[-1])
+
+    def extra_repr(self) -> str:
+        return (f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}, "
+                f"group_size={self.group_size}, zero_points={self.weight_zero is not None}, epilogue={self.epilogue}")
+
+
+# ---------------------------------------------------------------------------------------
 #  Model surgery (reference: quantize_utils.py:374-498)
 # ---------------------------------------------------------------------------------------
 def quantize_model_tensorcore(model, min_features=128, verbose=True):
@@ -630,6 +946,32 @@ def quantize_model_mixed(model, min_features=128, sparse_min_k=None, verbose=Tru
     if verbose:
         print(f"  Quantized {stats['num_replaced']} Linear layers: {stats['sparse_layers']} sparse, "
               f"{stats['dense_layers']} dense")
+    return stats
+
+
+def quantize_model_int4(model, min_features=128, group_size=64, symmetric=True, choose=None, verbose=True):
+    """Replace ``nn.Linear`` layers with ``Int4Linear`` in place: those of at least ``min_features`` inputs and outputs that
+    the layer's shape rules admit and, with ``choose``, those for which ``choose(name, layer)`` is true -- the ones that see
+    few rows (in the texture UNet ``lambda name, _: "time_emb" in name``); the other converters then take the rest."""
+    stats = {"total_params": 0, "quantized_params": 0, "skipped_params": 0, "num_replaced": 0, "kept_fp16": 0}
+    for name, child in list(model.named_modules()):
+        if not isinstance(child, nn.Linear) or not name:
+            continue
+        num_params = child.in_features * child.out_features
+        stats["total_params"] += num_params
+        if child.in_features < min_features or child.out_features < min_features:
+            stats["skipped_params"] += num_params
+        elif (child.in_features % 64 or child.out_features % 16 or child.in_features % group_size
+              or (choose is not None and not choose(name, child))):
+            stats["kept_fp16"] += 1
+        else:
+            parent = model.get_submodule(name.rpartition(".")[0])
+            setattr(parent, name.rpartition(".")[2], Int4Linear.from_linear(child, group_size, symmetric))
+            stats["quantized_params"] += num_params
+            stats["num_replaced"] += 1
+    if verbose:
+        print(_summary(stats, f"4-bit weights, groups of {group_size}", bytes_per_weight=0.5 + (2 if symmetric else 3) / group_size)
+              .replace("Int8Linear", "Int4Linear"))
     return stats
 
 

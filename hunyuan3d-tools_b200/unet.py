@@ -88,6 +88,8 @@ def _residual_norm(norm, x, h):
         got = (_qu._NATIVE or _qu._load_native()).norm_call(norm, x, h)
         if got is not None:
             return got
+    if isinstance(norm, _qu.AddRMSNorm):
+        return norm(x, h)
     x = x + h
     return x, norm(x)
 
@@ -199,6 +201,10 @@ class Attention(nn.Module):
 
     # (stacked k / v projections of all blocks, first column, last column + 1), set by fuse_context_projections
     _kv_slice = None
+    # a rotary.RotaryPositions that turns q and k, and its positions by number of tokens (None: counted); set by
+    # use_multiview_rotary, self-attention only
+    rotary = None
+    rotary_positions = None
 
     def forward(self, x, context=None, kv=None):
         """``kv``: keys and values of the context side by side, where the caller has them already."""
@@ -219,8 +225,12 @@ class Attention(nn.Module):
                 k, v = self.to_kv(context).split(c, dim=-1)
             else:
                 k, v = self.to_k(context), self.to_v(context)
-        q = q.view(b, n, self.heads, c // self.heads).transpose(1, 2)
-        k = k.view(b, m, self.heads, c // self.heads).transpose(1, 2)
+        q = q.view(b, n, self.heads, c // self.heads)
+        k = k.view(b, m, self.heads, c // self.heads)
+        if self.rotary is not None:       # both are this call's own: turned where they lie
+            at = None if self.rotary_positions is None else self.rotary_positions[n]
+            q, k = self.rotary(q, k, at, inplace=True)
+        q, k = q.transpose(1, 2), k.transpose(1, 2)
         v = v.view(b, m, self.heads, c // self.heads).transpose(1, 2)
         o = F.scaled_dot_product_attention(q, k, v)
         return self.to_out(o.transpose(1, 2).reshape(b, n, c))
@@ -397,8 +407,9 @@ class UNetSD21MV(nn.Module):
         names = {id(m): name for name, m in self.named_modules()}
         for attr, parts in (("time_proj_all", [names[id(m)] + ".time_emb_proj." for m in self._resnets()]),
                             ("context_proj_all", [names[id(m.block.attn2)] + ".to_kv." for m in self._transformers()])):
-            if isinstance(getattr(self, attr, None), _qu.Int8Linear):
-                _qu.Int8Linear.concat_state(state_dict, prefix + attr + ".", [prefix + part for part in parts])
+            layer = getattr(self, attr, None)
+            if isinstance(layer, (_qu.Int8Linear, _qu.Int4Linear)):
+                layer.concat_state(state_dict, prefix + attr + ".", [prefix + part for part in parts])
         super()._load_from_state_dict(state_dict, prefix, *args)
 
     def use_channels_last(self) -> "UNetSD21MV":
@@ -461,26 +472,51 @@ class UNetSD21MV(nn.Module):
 
 
 def fuse_geglu_layers(model: nn.Module) -> int:
-    """Switches every ``Int8Linear`` GEGLU up-projection (dense or 2:4 sparse) to the fused
+    """Switches every ``Int8Linear`` (dense or 2:4 sparse) or ``Int4Linear`` GEGLU up-projection to the fused
     ``value * gelu(gate)`` epilogue (rows interleaved offline).  Returns the number fused."""
-    from .quantize_utils import Int8Linear
+    from .quantize_utils import Int4Linear, Int8Linear
     n = 0
     for m in model.modules():
         if isinstance(m, GEGLUFeedForward) and isinstance(m.proj, Int8Linear) \
                 and m.proj.mode in ("tc", "sparse") and m.proj.epilogue == "linear":
             m.proj.interleave_geglu_rows()
             n += 1
+        elif isinstance(m, GEGLUFeedForward) and isinstance(m.proj, Int4Linear) and m.proj.epilogue == "linear":
+            m.proj.interleave_geglu_rows()
+            n += 1
     return n
 
 
+def use_multiview_rotary(model: nn.Module, positions: dict, base: float = 10000.0, interleaved: bool = True, scaling=None) -> int:
+    """Gives every multiview attention rotary positions: ``positions`` maps a number of tokens (views x height x width of a
+    level) to an int tensor (tokens) or (tokens, axes), such as (view, row, column) or a voxel's coordinates.  The head's
+    dimensions are shared out evenly among the axes.  Returns the number of attentions changed."""
+    from .rotary import RotaryPositions
+    ends = {t.shape[1] if t.dim() == 2 else 1 for t in positions.values()}
+    if len(ends) != 1 or any(t.shape[0] != n for n, t in positions.items()):
+        raise RuntimeError("positions must map each number of tokens to that many positions, all of the same axes")
+    axes, count = ends.pop(), 0
+    for blk in model.modules():
+        if not isinstance(blk, TransformerBlock) or blk.num_views < 2:
+            continue
+        attn = blk.attn_mv
+        dim = blk.norm_mv.normalized_shape[0] // attn.heads
+        pairs = dim // 2
+        parts = [2 * (pairs // axes + (1 if i < pairs % axes else 0)) for i in range(axes)]
+        attn.rotary = RotaryPositions(dim, sum(parts), base, interleaved, parts, scaling)
+        attn.rotary_positions = dict(positions)
+        count += 1
+    return count
+
+
 def fuse_layernorm_quant(model: nn.Module) -> int:
-    """Replaces the LayerNorms of every transformer block whose consumers are all
+    """Replaces the LayerNorms (RMSNorms: by ``Int8RMSNorm``) of every transformer block whose consumers are all
     ``Int8Linear`` layers by ``Int8LayerNorm``: norm1 -> stacked q/k/v, norm_mv -> stacked
     multiview q/k/v, norm2 -> cross-attention q, norm3 -> FFN up-projection.  Each of those
     projections then starts from int8 codes emitted by the normalisation kernel instead of
     re-reading and re-quantising its bf16 output.  Run after ``fuse_qkv_layers``.  Returns the
     number of LayerNorms converted."""
-    from .quantize_utils import Int8Linear, Int8LayerNorm
+    from .quantize_utils import Int8Linear, Int8LayerNorm, Int8RMSNorm
     n = 0
     for blk in model.modules():
         if not isinstance(blk, TransformerBlock):
@@ -491,8 +527,8 @@ def fuse_layernorm_quant(model: nn.Module) -> int:
                  ("norm3", [blk.ff.proj])]
         for name, consumers in pairs:
             norm = getattr(blk, name)
-            if isinstance(norm, nn.LayerNorm) and all(isinstance(c, Int8Linear) for c in consumers):
-                setattr(blk, name, Int8LayerNorm(norm))
+            if isinstance(norm, (nn.LayerNorm, nn.RMSNorm)) and all(isinstance(c, Int8Linear) for c in consumers):
+                setattr(blk, name, Int8LayerNorm(norm) if isinstance(norm, nn.LayerNorm) else Int8RMSNorm(norm))
                 n += 1
     return n
 
@@ -523,11 +559,12 @@ def fuse_qkv_layers(model: nn.Module) -> int:
 
 def _stack(layers):
     """One layer of all of them, or None where they cannot be stacked."""
-    from .quantize_utils import Int8Linear
-    if not layers or not all(type(l) is Int8Linear and l.epilogue == "linear" for l in layers):
+    from .quantize_utils import Int4Linear, Int8Linear
+    kind = type(layers[0]) if layers else None
+    if kind not in (Int8Linear, Int4Linear) or not all(type(l) is kind and l.epilogue == "linear" for l in layers):
         return None
     try:
-        return Int8Linear.concat(layers)
+        return kind.concat(layers)
     except RuntimeError:        # of different modes, types or inputs
         return None
 

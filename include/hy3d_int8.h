@@ -153,6 +153,62 @@ int hy3d_add_layernorm_quantize(const void* x, const void* add, void* sum, int x
                                 void* stream);
 
 /*
+ * Root-mean-square norm over the last dimension, optionally of x + add, into 16-bit values, int8 codes with per-token
+ * scales, or both:
+ *   t = add ? round(x + add) : x;  y = round(t * rstd * gamma), rstd = 1 / sqrt(sum(t^2) / K + eps)
+ *   scale = max(max|y|, 1e-8) / 127;  q = rint(y / scale)      -- equal to hy3d_quantize_rows(y) bit for bit
+ * x, add: (M,K) f16 / bf16 with row pitches ldx and ld_add (elements, multiples of 8); add may be NULL.  sum (M,K)
+ * receives t where there is an add (it may be x or add themselves if their pitch is K).  y (M,K) or NULL; q (M,K) and
+ * scale (M) or NULL; at least one of y and q.  gamma: (K) of g_dtype (f16 / bf16 / f32) or NULL (1).  The statistics are
+ * fp32 sums in an order that K alone fixes.  A row with a NaN or an infinity: y has NaN there as the formula gives it, and
+ * the scale is NaN or infinite, so that every value of the row is NaN.  Requires K % 8 == 0, K <= 16384, 16-byte aligned
+ * rows and gamma.  No counterpart in the reference, whose UNet has LayerNorms only.
+ */
+int hy3d_rmsnorm(const void* x, int64_t ldx, const void* add, int64_t ld_add, void* sum, int x_dtype, int64_t M, int64_t K,
+                 const void* gamma, int g_dtype, float eps, void* y, int8_t* q, float* scale, void* stream);
+
+/* y = round(q * scale) per row: the values that int8 codes stand for, (M,K) f16 / bf16.  K % 8 == 0, y 16-byte aligned. */
+int hy3d_dequantize_rows(const int8_t* q, const float* scale, int64_t M, int64_t K, int out_dtype, void* y, void* stream);
+
+/*
+ * Rotary positions.  The first `rot` dimensions of every head are rot / 2 pairs -- (i, i + rot / 2), or (2i, 2i + 1) where
+ * interleaved -- and pair i turns by the angle position[axis[i]] * turns[i] / 2^64 of a full turn (inverse: by minus that):
+ *   (u, v) -> (u cos a - v sin a, v cos a + u sin a) * amplitude, computed in fp32 and rounded once
+ * The other dimensions are copied.  turns and axis are HOST arrays of rot / 2 entries; the product with the position is
+ * taken modulo 2^64, which is modulo one turn, so the angle is exact at any position.
+ * One or two sides (queries, keys) of `batch` sequences of n tokens, each with its own number of heads and strides (in
+ * elements; the head's dimensions are adjacent).  dst == src with the same strides turns in place; other overlaps are the
+ * caller's error.  positions: int64 or int32 device array, element of (b, token, axis) at b * pb + token * pn + axis * pa,
+ * or NULL for offset + token.  rot even, <= dim and <= 512; any alignment (16-byte vectors where everything allows them).
+ * No counterpart in the reference.
+ */
+typedef struct hy3d_rotary_side {
+  const void* src;
+  void* dst;
+  int64_t src_b, src_n, src_h, dst_b, dst_n, dst_h;
+  int heads;
+} hy3d_rotary_side;
+int hy3d_rotary(const hy3d_rotary_side* sides, int n_sides, int dtype, int64_t batch, int64_t n, int dim, int rot, int interleaved,
+                const void* positions, int positions_64, int64_t pb, int64_t pn, int64_t pa, int64_t offset,
+                const uint64_t* turns, const uint8_t* axis, float amplitude, int inverse, void* stream);
+
+/*
+ * Linear layer with 4-bit weights, group scales and 16-bit activations:
+ *   y[m,n] = epilogue( sum_g scale[n,g] * sum_{k in group g} x[m,k] * (code[n,k] - zero[n,g]) + bias[n] )
+ * with fp32 sums of exact products and one rounding to x's type.  x: (M,K) f16 / bf16, row pitch ldx (a multiple of 8).
+ * w: codes 0..15 in tiles of 16 rows x 64 columns, [N/16][K/64][lane][4 words]: lane 4g + t holds rows g and g + 8; words 0
+ * and 2 are row g's columns 8t .. 8t+7 and 32 + 8t ..., words 1 and 3 row g + 8's; nibble j < 4 of a word is column 2j,
+ * nibble 4 + j column 2j + 1.  scale: f16 / bf16 [N/16][K/group][16], place 2g for row g and 2g + 1 for row g + 8.  zero: the
+ * same places, a byte 0..15 each, or NULL for 8 throughout.  group: 32, or a multiple of 64; divides K.  bias (N) or NULL.
+ * Epilogues as for the int8 GEMMs (HY3D_EPI_GEGLU: rows interleaved in blocks of 16, N / 2 columns out), GELU in its exact
+ * form.  out: (M, N or N / 2) of x's type.  Requires K % 64 == 0, N % 16 == 0 (% 32 GEGLU), 16-byte aligned x rows and w.
+ * No workspace.  No counterpart in the reference.
+ */
+int hy3d_linear_w4(const void* x, int x_dtype, int64_t ldx, const void* w, const void* scale, int scale_dtype, const void* zero,
+                   int64_t group, const void* bias, int bias_dtype, void* out, int64_t M, int64_t N, int64_t K, int epilogue,
+                   void* stream);
+
+/*
  * Self-check of the GELU that the GEMM epilogues evaluate (test hook, no reference counterpart): compares it on the
  * device with 0.5 * g * (1 + erf(g / sqrt 2)) in fp32 for every fp32 g of magnitude 2^-125 and up, and counts the
  * values where the two are further apart than bound * |g|.  The bf16 GEGLU epilogue rounds as that form does because
