@@ -589,8 +589,8 @@ _NIBBLE_COLUMNS = (0, 2, 4, 6, 1, 3, 5, 7)
 def _pack_codes(codes: torch.Tensor) -> torch.Tensor:
     """Codes (N,K) of 0..15 -> (N/16, K/64, 512) bytes in the order of csrc/linear_w4.cu."""
     n, k = codes.shape
-    c = codes.to(torch.uint8).view(n // 16, 2, 8, k // 64, 2, 4, 8)          # row block, half, g, tile, sub, t, column
-    c = c.permute(0, 3, 2, 5, 4, 1, 6)[..., list(_NIBBLE_COLUMNS)]           # row block, tile, g, t, sub, half, nibble
+    c = codes.to(torch.uint8).view(n // 16, 2, 8, k // 64, 2, 2, 4, 4)       # row block, half, g, tile, sub, 16s, t, column
+    c = c.permute(0, 3, 2, 6, 4, 1, 5, 7).flatten(-2)[..., list(_NIBBLE_COLUMNS)]      # row block, tile, g, t, sub, half, nibble
     return (c[..., 0::2] | c[..., 1::2] << 4).reshape(n // 16, k // 64, 512)
 
 
@@ -599,7 +599,8 @@ def _unpack_codes(packed: torch.Tensor) -> torch.Tensor:
     p = packed.view(blocks, tiles, 8, 4, 2, 2, 4)
     c = torch.stack([p & 15, p >> 4], dim=-1).flatten(-2)
     inverse = [_NIBBLE_COLUMNS.index(i) for i in range(8)]
-    return c[..., inverse].permute(0, 5, 2, 1, 4, 3, 6).reshape(blocks * 16, tiles * 64)
+    c = c[..., inverse].unflatten(-1, (2, 4))               # row block, tile, g, t, sub, half, 16s, column
+    return c.permute(0, 5, 2, 1, 4, 6, 3, 7).reshape(blocks * 16, tiles * 64)
 
 
 def _pack_groups(v: torch.Tensor) -> torch.Tensor:
@@ -621,7 +622,7 @@ class Int4Linear(nn.Module):
 
     Products are exact and sums fp32, the scale multiplies a group's sum, and the output is rounded once.  Stands beside
     ``Int8Linear`` (same epilogues, ``concat``, ``interleave_geglu_rows``, checkpoints); the reference has no counterpart.
-    Any number of rows; in_features % 64 == 0, out_features % 16 == 0, groups of 32 or of a multiple of 64 columns that
+    Any number of rows; in_features % 64 == 0 and at most 32768, out_features % 16 == 0, groups of 32 or of a multiple of 64 columns that
     divides in_features.  CUDA fp16 / bf16 only; no gradient is recorded.
 
     Buffers: ``weight_int4`` (N/16, K/64, 512) uint8, ``weight_scale`` (N/16, groups, 16), ``weight_zero`` likewise uint8 or
@@ -632,8 +633,8 @@ class Int4Linear(nn.Module):
     def __init__(self, in_features: int, out_features: int, bias: bool = True, dtype: torch.dtype = torch.float16,
                  group_size: int = 64, symmetric: bool = True):
         super().__init__()
-        if in_features <= 0 or out_features <= 0 or in_features % 64 or out_features % 16:
-            raise RuntimeError("Int4Linear needs in_features % 64 == 0 and out_features % 16 == 0, "
+        if in_features <= 0 or out_features <= 0 or in_features % 64 or out_features % 16 or in_features > 32768:
+            raise RuntimeError("Int4Linear needs in_features % 64 == 0, at most 32768, and out_features % 16 == 0, "
                                f"got {in_features} and {out_features}")
         if group_size < 32 or (group_size != 32 and group_size % 64) or in_features % group_size:
             raise RuntimeError("Int4Linear needs groups of 32 or of a multiple of 64 columns that divides in_features, "
@@ -961,7 +962,7 @@ def quantize_model_int4(model, min_features=128, group_size=64, symmetric=True, 
         stats["total_params"] += num_params
         if child.in_features < min_features or child.out_features < min_features:
             stats["skipped_params"] += num_params
-        elif (child.in_features % 64 or child.out_features % 16 or child.in_features % group_size
+        elif (child.in_features % 64 or child.out_features % 16 or child.in_features > 32768 or child.in_features % group_size
               or (choose is not None and not choose(name, child))):
             stats["kept_fp16"] += 1
         else:

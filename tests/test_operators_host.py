@@ -28,7 +28,8 @@ def test_packed_codes_are_where_the_header_says(qu):
     words = words[..., 0] | words[..., 1] << 8 | words[..., 2] << 16 | words[..., 3] << 24
     for rb, tile, lane, word, nibble in [(0, 0, 0, 0, 0), (2, 1, 31, 3, 7), (1, 2, 13, 1, 5), (0, 2, 6, 2, 3), (2, 0, 17, 0, 4)]:
         row = rb * 16 + lane // 4 + 8 * (word & 1)
-        col = tile * 64 + 32 * (word >> 1) + 8 * (lane % 4) + (2 * nibble if nibble < 4 else 2 * (nibble - 4) + 1)
+        i = 2 * nibble if nibble < 4 else 2 * (nibble - 4) + 1
+        col = tile * 64 + 32 * (word >> 1) + 16 * (i >> 2) + 4 * (lane % 4) + (i & 3)
         assert int(words[rb, tile, lane, word] >> (4 * nibble) & 15) == int(codes[row, col])
     assert torch.equal(qu._unpack_codes(qu._pack_codes(codes)), codes)
     v = torch.randn(48, 5, generator=g)
