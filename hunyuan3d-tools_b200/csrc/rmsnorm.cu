@@ -57,9 +57,8 @@ struct Args {
   int K, lg, g_dtype;
 };
 
-// Eight of gamma's values as pairs.
-template <bool kBf16>
-__device__ __forceinline__ void load_gamma(const Args& a, int vec, float2 (&g)[4]) {
+// Eight of gamma's values as pairs; `raw` are the 16-bit ones, loaded earlier.
+__device__ __forceinline__ void gamma_pairs(const Args& a, int vec, const uint4& raw, float2 (&g)[4]) {
   if (!a.gamma) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) g[j] = make_float2(1.0f, 1.0f);
@@ -69,9 +68,8 @@ __device__ __forceinline__ void load_gamma(const Args& a, int vec, float2 (&g)[4
     g[0] = make_float2(u.x, u.y); g[1] = make_float2(u.z, u.w);
     g[2] = make_float2(v.x, v.y); g[3] = make_float2(v.z, v.w);
   } else {
-    const uint4 w = __ldg(reinterpret_cast<const uint4*>(a.gamma) + vec);
     float f[8];
-    if (a.g_dtype == HY3D_BF16) unpack8<true>(w, f); else unpack8<false>(w, f);
+    if (a.g_dtype == HY3D_BF16) unpack8<true>(raw, f); else unpack8<false>(raw, f);
 #pragma unroll
     for (int j = 0; j < 4; ++j) g[j] = make_float2(f[2 * j], f[2 * j + 1]);
   }
@@ -79,8 +77,15 @@ __device__ __forceinline__ void load_gamma(const Args& a, int vec, float2 (&g)[4
 
 // 2^lg threads share a row, each with up to kV 16-byte vectors that stay in registers between the statistics and the
 // output.  A block holds blockDim >> lg rows; threads past the last row compute it too and store nothing.
-template <bool kBf16, int kV, bool kAdd, bool kCodes>
-__global__ void __launch_bounds__(512)
+// Bound by HBM with a residual (12288 x 640 to 16 bits 9.3 us, 6.7 TB/s; to codes 10.7, 5.1; 8192 x 8192 to 16 bits 81.3,
+// 6.6).  Without one, to codes, by the chain of load, two reductions and store with too few rows in flight (3855 x 1536 7.9 us,
+// 2.2 TB/s; 49152 x 320 13.9, 3.4); blocks per SM follow from the registers kV needs, none of which may spill: with three
+// blocks for every kV those two took 8.6 and 14.8.  (A grid-stride loop that requests the next row ahead of the current
+// one's work spilled: 12288 x 640 10.8 -> 13.2.)
+// gamma's 16-bit values are requested with the row's, not after its statistics, where there are registers for both: one row
+// of 4096 3.2 -> 2.5 us.
+template <bool kBf16, int kV, bool kAdd, bool kCodes, bool kWide>
+__global__ void __launch_bounds__(kWide ? 512 : kThreads, kWide ? 2 : kV == 1 ? 6 : kV == 2 ? 5 : kV == 3 ? 4 : 3)
 rmsnorm_kernel(const __grid_constant__ Args a) {
   __shared__ float s_part[2][16];
   pdl_launch_dependents();
@@ -109,6 +114,12 @@ rmsnorm_kernel(const __grid_constant__ Args a) {
       if (live && sub + i * G < nvec) dst[i * G] = v[i];
     }
   }
+  constexpr bool kEarly = !kCodes || kV <= (kWide ? 3 : 4);
+  uint4 graw[kV];
+  if (kEarly && a.gamma && a.g_dtype != HY3D_F32)
+#pragma unroll
+    for (int i = 0; i < kV; ++i)
+      graw[i] = sub + i * G < nvec ? __ldg(reinterpret_cast<const uint4*>(a.gamma) + sub + i * G) : make_uint4(0, 0, 0, 0);
   float2 ss2 = make_float2(0.0f, 0.0f);
 #pragma unroll
   for (int i = 0; i < kV; ++i) {
@@ -136,7 +147,8 @@ rmsnorm_kernel(const __grid_constant__ Args a) {
   for (int i = 0; i < kV; ++i) {
     if (sub + i * G < nvec) {
       float2 g[4];
-      load_gamma<kBf16>(a, sub + i * G, g);
+      if (!kEarly && a.gamma && a.g_dtype != HY3D_F32) graw[i] = __ldg(reinterpret_cast<const uint4*>(a.gamma) + sub + i * G);
+      gamma_pairs(a, sub + i * G, graw[i], g);
       float f[8];
       unpack8<kBf16>(v[i], f);
       uint32_t w[4];
@@ -163,14 +175,17 @@ rmsnorm_kernel(const __grid_constant__ Args a) {
     const RowQuant rq = row_quant(amax);
     if (live && sub == 0) a.scale[row] = amax == amax ? rq.scale : amax;
     uint2* dst = reinterpret_cast<uint2*>(a.q + row * static_cast<int64_t>(a.K)) + sub;
+    auto write = [&](auto exact) {
 #pragma unroll
-    for (int i = 0; i < kV; ++i) {
-      if (live && sub + i * G < nvec) {
-        float f[8];
-        unpack8<kBf16>(v[i], f);
-        dst[i * G] = quant8(f, rq);
+      for (int i = 0; i < kV; ++i) {
+        if (live && sub + i * G < nvec) {
+          float f[8];
+          unpack8<kBf16>(v[i], f);
+          dst[i * G] = quant8<decltype(exact)::value>(f, rq);
+        }
       }
-    }
+    };
+    if (rq.exact) write(quant::True{}); else write(quant::False{});
   }
 }
 
@@ -178,10 +193,13 @@ template <bool kBf16>
 int launch(const Args& in, cudaStream_t stream) {
   Args a = in;
   const int nvec = a.K >> 3;
-  // Threads per row: the fewest (a power of two) that hold it with 5 vectors each.  By K alone: the number of threads
-  // fixes the order of the row's sum, so a row's result does not depend on how many others there are.
+  // Threads per row: the fewest (a power of two, eight where the row has as many vectors, so that a load touches whole 128-byte
+  // lines: 30000 x 64 5.6 -> 3.8 us) that hold it with 4 vectors each; eight threads take 5.  More vectors a thread and fewer
+  // threads save reductions and barriers (at most 3 vectors: 5000 x 2048 to codes 11.9 -> 14.1 us, 49152 x 320 13.9 -> 16.4),
+  // fewer vectors leave registers for more blocks on an SM (5: 12288 x 640 to 16 bits 9.3 -> 10.1).  By K alone: the number
+  // of threads fixes the order of the row's sum, so a row's result does not depend on how many others there are.
   a.lg = 0;
-  while (((nvec + (1 << a.lg) - 1) >> a.lg) > 5) ++a.lg;
+  while ((a.lg < 3 && (1 << a.lg) < nvec) || ((nvec + (1 << a.lg) - 1) >> a.lg) > (a.lg == 3 ? 5 : 4)) ++a.lg;
   const int v = (nvec + (1 << a.lg) - 1) >> a.lg;
   const int threads = a.lg > 8 ? 1 << a.lg : kThreads;
   const int rows = threads >> a.lg;
@@ -191,43 +209,53 @@ int launch(const Args& in, cudaStream_t stream) {
   cfg.gridDim = dim3(static_cast<unsigned>(blocks));
   cfg.blockDim = dim3(threads);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1] = {pdl_attribute()};
+  cudaLaunchAttribute attr[2] = {pdl_attribute(), carveout_attribute(4, 128)};
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   using KernelFn = void (*)(const Args);
-#define HY3D_RMS(V)                                                                    \
-  {{rmsnorm_kernel<kBf16, V, false, false>, rmsnorm_kernel<kBf16, V, false, true>},    \
-   {rmsnorm_kernel<kBf16, V, true, false>, rmsnorm_kernel<kBf16, V, true, true>}}
-  static const KernelFn kernels[5][2][2] = {HY3D_RMS(1), HY3D_RMS(2), HY3D_RMS(3), HY3D_RMS(4), HY3D_RMS(5)};
+#define HY3D_RMS(V, W)                                                                      \
+  {{rmsnorm_kernel<kBf16, V, false, false, W>, rmsnorm_kernel<kBf16, V, false, true, W>},   \
+   {rmsnorm_kernel<kBf16, V, true, false, W>, rmsnorm_kernel<kBf16, V, true, true, W>}}
+  static const KernelFn kernels[5][2][2] = {HY3D_RMS(1, false), HY3D_RMS(2, false), HY3D_RMS(3, false), HY3D_RMS(4, false),
+                                            HY3D_RMS(5, false)};
+  static const KernelFn wide[2][2][2] = {HY3D_RMS(3, true), HY3D_RMS(4, true)};      // 512 threads: K from 8200 on, 3 or 4 vectors each
 #undef HY3D_RMS
-  if (cudaLaunchKernelEx(&cfg, kernels[v - 1][a.add ? 1 : 0][a.q ? 1 : 0], a) != cudaSuccess) {
+  const KernelFn kernel = a.lg > 8 ? wide[v - 3][a.add ? 1 : 0][a.q ? 1 : 0] : kernels[v - 1][a.add ? 1 : 0][a.q ? 1 : 0];
+  if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) {
     cudaGetLastError();
     return HY3D_ERR_CUDA;
   }
   return HY3D_OK;
 }
 
-// Codes back to the values they stand for: round16(q * scale).
+// Codes back to the values they stand for: round16(q * scale).  A block takes kUnroll * kThreads adjacent vectors of eight;
+// a vector's row comes from one division per thread and additions from there on.
 __global__ void __launch_bounds__(kThreads)
 dequantize_rows_kernel(const uint2* __restrict__ q, const float* __restrict__ scale, uint4* __restrict__ y, int64_t total,
                        int vec_cols, int out_dtype) {
   pdl_launch_dependents();
   constexpr int kUnroll = 4;
-  const int64_t base = static_cast<int64_t>(blockIdx.x) * (kUnroll * kThreads) + threadIdx.x;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * (kUnroll * kThreads) + threadIdx.x;
+  int64_t row = total <= 0xFFFFFFFFll ? static_cast<int64_t>(static_cast<uint32_t>(first) / static_cast<uint32_t>(vec_cols)) : first / vec_cols;
+  int col = static_cast<int>(first - row * vec_cols);
+  const int step_row = kThreads / vec_cols, step_col = kThreads - step_row * vec_cols;
   pdl_wait();
   uint2 v[kUnroll];
   float s[kUnroll];
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    const int64_t at = base + u * kThreads;
+    const int64_t at = first + u * kThreads;
     if (at < total) {
       v[u] = __ldcs(q + at);
-      s[u] = __ldg(scale + at / vec_cols);
+      s[u] = __ldg(scale + row);
     }
+    row += step_row;
+    col += step_col;
+    if (col >= vec_cols) { col -= vec_cols; ++row; }
   }
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    const int64_t at = base + u * kThreads;
+    const int64_t at = first + u * kThreads;
     if (at < total) {
       const uint32_t w[2] = {v[u].x, v[u].y};
       uint32_t o[4];
