@@ -5,7 +5,13 @@
 // The angle is exact at any position: w_i comes as a 64-bit fraction of a turn, 2^64 w_i / (2 pi), so the product with
 // the integer position is the angle modulo one turn by itself -- the integer product wraps where the circle does.  Its
 // error is position * 2^-65 turns; the fp32 product position * w_i would be off by 0.06 radians at a million.  There is
-// no table of cosines to build, to keep or to outgrow.
+// no table of cosines to build, to keep or to outgrow.  The angle's top two bits are its quadrant, and the rest is small
+// enough for the Taylor polynomials of sine and cosine.
+//
+// Bound by HBM: 4 bytes of traffic per value (32768 tokens of 40 heads of 128: 106.8 us, 6.3 TB/s; 8 x 1 tokens: 2.6 us).
+// A thread has the sines and cosines of 8 pairs and turns those of up to 8 heads with them, loads of four heads in flight at
+// a time: one head after the other with sincospif took 146 and 3.4.  With three axes (2 x 6144 tokens of 20 heads of 64: 15.9,
+// 4.0 TB/s) a thread waits for its positions before its sines, and has fewer heads to use them for.
 #include "common.cuh"
 
 namespace hy3d {
@@ -29,17 +35,18 @@ struct Args {
   int64_t tokens;                 // batch * n
   uint32_t n;                     // tokens of a sequence
   int heads0, heads;              // of the first side, of both
-  int units, units_all;           // rotated units of a head, and with those that are only copied
+  int units, tail_units;          // of a head: turned, and only copied
+  uint32_t turn_blocks;           // blocks that turn; the others copy
   int lanes_h;                    // threads of a token that share a unit's heads
   int half, dim;                  // rotated pairs; dimensions of a head
   float amplitude;
-  uint8_t pos64, inverse, small;
+  uint8_t pos64, inverse, small, one_axis;
   uint8_t axis[kMaxPairs];
   uint64_t turns[kMaxPairs];
 };
 
-// kP pairs per unit.  Half layout: kP elements at 2 places, half apart; interleaved: 2 kP adjacent elements.  With one
-// pair nothing is known of the alignment, and elements are moved one by one.
+// kP pairs per unit: kP elements at 2 places, half apart, in both layouts -- interleaved, each of the two vectors holds
+// kP / 2 whole pairs.  With one pair nothing is known of the alignment, and its elements are moved one by one.
 template <int kBytes>
 __device__ __forceinline__ void copy_in(uint32_t* w, const uint16_t* p) {
   if (kBytes == 2) w[0] = *p;
@@ -70,15 +77,49 @@ __device__ __forceinline__ float2 widen(uint32_t w) {
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
-// A thread has one unit of one token and walks over that token's heads, lanes_h apart: the sines and cosines are
-// computed once for all of them.  Neighbouring threads have neighbouring units, then neighbouring heads.
+// Sine and cosine of a 64-bit fraction of a turn, whose top 32 bits are given: x = angle past the nearest quarter turn,
+// |x| <= pi / 4, where the next terms are below 2e-9 (sine, relative) and 3e-8 (cosine).
+__device__ __forceinline__ void sincos_turn(uint32_t phase, float& s, float& c) {
+  const uint32_t shifted = phase + 0x20000000u, quadrant = shifted >> 30;
+  const float x = static_cast<float>(static_cast<int32_t>(shifted & 0x3FFFFFFFu) - 0x20000000) * 1.4629180792671596e-9f;     // 2 pi / 2^32
+  const float y = x * x;
+  float sine = fmaf(y, 2.7557319e-6f, -1.9841270e-4f), cosine = fmaf(y, 2.4801587e-5f, -1.3888889e-3f);
+  sine = fmaf(sine, y, 8.3333333e-3f);
+  cosine = fmaf(cosine, y, 4.1666667e-2f);
+  sine = fmaf(sine, y, -1.6666667e-1f);
+  cosine = fmaf(cosine, y, -0.5f);
+  sine = fmaf(sine * y, x, x);
+  cosine = fmaf(cosine, y, 1.0f);
+  const bool swap = quadrant & 1;
+  s = swap ? cosine : sine;
+  c = swap ? sine : cosine;
+  s = __uint_as_float(__float_as_uint(s) ^ (quadrant & 2) << 30);
+  c = __uint_as_float(__float_as_uint(c) ^ ((quadrant + 1) & 2) << 30);
+}
+
+constexpr int kBatch = 4;         // heads whose loads are in flight together
+
+// The first blocks turn: a thread has one unit of one token and walks over that token's heads, lanes_h apart.
+// Neighbouring threads have neighbouring units, then neighbouring heads.  The blocks behind them copy the dimensions that
+// are not turned, in the same order.
 template <bool kBf16, bool kInterleaved, int kP>
 __global__ void __launch_bounds__(kThreads)
 rotary_kernel(const __grid_constant__ Args a) {
+  __shared__ uint64_t s_turns[kMaxPairs];
+  __shared__ uint8_t s_axis[kMaxPairs];
   pdl_launch_dependents();
   constexpr int kType = kBf16 ? HY3D_BF16 : HY3D_F16;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const uint32_t per_token = static_cast<uint32_t>(a.lanes_h * a.units_all);
+  const bool copies = blockIdx.x >= a.turn_blocks;
+  if (!copies) {                  // indexed by lane, the parameter itself would be read one address after the other
+    for (int i = threadIdx.x; i < a.half; i += kThreads) {
+      s_turns[i] = a.turns[i];
+      s_axis[i] = a.axis[i];
+    }
+    __syncthreads();
+  }
+  const int units = copies ? a.tail_units : a.units;
+  const int64_t id = static_cast<int64_t>(copies ? blockIdx.x - a.turn_blocks : blockIdx.x) * kThreads + threadIdx.x;
+  const uint32_t per_token = static_cast<uint32_t>(a.lanes_h * units);
   int64_t token, b;
   if (a.small) {                  // a 64-bit division costs as much as the sines
     token = static_cast<uint32_t>(id) / per_token;
@@ -89,78 +130,96 @@ rotary_kernel(const __grid_constant__ Args a) {
   }
   if (token >= a.tokens) return;
   const uint32_t rest = static_cast<uint32_t>(id - token * per_token);
-  const int first_head = rest / a.units_all, unit = rest - first_head * a.units_all;
+  const int first_head = rest / units, unit = rest - first_head * units;
   const uint32_t n = static_cast<uint32_t>(token - b * a.n);
   pdl_wait();
+  auto source = [&](int h) {
+    const Side& s = a.side[h >= a.heads0];
+    return s.src + b * s.sb + n * s.sn + (h >= a.heads0 ? h - a.heads0 : h) * s.sh;
+  };
+  auto target = [&](int h) {
+    const Side& s = a.side[h >= a.heads0];
+    return s.dst + b * s.db + n * s.dn + (h >= a.heads0 ? h - a.heads0 : h) * s.dh;
+  };
 
-  if (unit >= a.units) {          // dimensions behind the rotated ones
-    const int at = 2 * a.half + (unit - a.units) * 2 * kP;
-    for (int h = first_head; h < a.heads; h += a.lanes_h) {
-      const Side& s = a.side[h >= a.heads0];
-      const int hh = h >= a.heads0 ? h - a.heads0 : h;
-      const uint16_t* src = s.src + b * s.sb + n * s.sn + hh * s.sh + at;
-      uint16_t* dst = s.dst + b * s.db + n * s.dn + hh * s.dh + at;
+  if (copies) {
+    const int at = 2 * a.half + unit * 2 * kP;
+    for (int h0 = first_head; h0 < a.heads; h0 += kBatch * a.lanes_h) {
       if (kP == 1) {
-        dst[0] = src[0];
-        if (at + 1 < a.dim) dst[1] = src[1];
+        for (int h = h0; h < a.heads && h < h0 + kBatch * a.lanes_h; h += a.lanes_h) {
+          target(h)[at] = source(h)[at];
+          if (at + 1 < a.dim) target(h)[at + 1] = source(h)[at + 1];
+        }
       } else {
-        uint32_t w[kP];
-        copy_in<4 * kP>(w, src);
-        copy_out<4 * kP>(dst, w);
+        uint32_t w[kBatch][kP];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+          if (h0 + j * a.lanes_h < a.heads) copy_in<4 * kP>(w[j], source(h0 + j * a.lanes_h) + at);
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+          if (h0 + j * a.lanes_h < a.heads) copy_out<4 * kP>(target(h0 + j * a.lanes_h) + at, w[j]);
       }
     }
     return;
   }
 
   float cs[kP], sn[kP];
+  const int at = kInterleaved && kP == 1 ? 2 * unit : unit * kP, apart = kInterleaved && kP == 1 ? 1 : a.half;
+  constexpr int kW = kP > 1 ? kP / 2 : 1;
+  for (int h0 = first_head; h0 < a.heads; h0 += kBatch * a.lanes_h) {
+    uint32_t u[kBatch][kW], v[kBatch][kW];         // the vectors at the two places
 #pragma unroll
-  for (int i = 0; i < kP; ++i) {
-    const int pair = unit * kP + i;
-    int64_t p = a.offset + n;
-    if (a.positions) {
-      const int64_t at = b * a.pb + n * a.pn + a.axis[pair] * a.pa;
-      p = a.pos64 ? static_cast<const int64_t*>(a.positions)[at] : static_cast<const int32_t*>(a.positions)[at];
+    for (int j = 0; j < kBatch; ++j) {
+      if (h0 + j * a.lanes_h >= a.heads) continue;
+      const uint16_t* src = source(h0 + j * a.lanes_h) + at;
+      copy_in<2 * kP>(u[j], src);
+      copy_in<2 * kP>(v[j], src + apart);
     }
-    const uint64_t phase = static_cast<uint64_t>(p) * a.turns[pair];                       // modulo one turn
-    const float t = static_cast<float>(static_cast<int32_t>(phase >> 32)) * 4.656612873077393e-10f;   // half turns, [-1, 1)
-    sincospif(t, &sn[i], &cs[i]);
-    cs[i] *= a.amplitude;
-    sn[i] *= a.inverse ? -a.amplitude : a.amplitude;
-  }
-  for (int h = first_head; h < a.heads; h += a.lanes_h) {
-    const Side& s = a.side[h >= a.heads0];
-    const int hh = h >= a.heads0 ? h - a.heads0 : h;
-    const uint16_t* src = s.src + b * s.sb + n * s.sn + hh * s.sh;
-    uint16_t* dst = s.dst + b * s.db + n * s.dn + hh * s.dh;
-    if (kInterleaved) {
-      uint32_t w[kP];
-      if (kP == 1) w[0] = src[unit * 2] | static_cast<uint32_t>(src[unit * 2 + 1]) << 16;
-      else copy_in<4 * kP>(w, src + unit * 2 * kP);
+    if (h0 == first_head) {                        // while the first loads are under way
+      const int64_t row = b * a.pb + n * a.pn;
+      int64_t p = a.offset + n;
+      int axis = -1;
 #pragma unroll
       for (int i = 0; i < kP; ++i) {
-        const float2 f = widen<kBf16>(w[i]);
-        w[i] = pack2(fmaf(f.x, cs[i], -f.y * sn[i]), fmaf(f.y, cs[i], f.x * sn[i]), kType);
+        const int pair = kInterleaved && kP > 1 ? unit * kW + i + (i < kW ? 0 : (a.half >> 1) - kW) : unit * kP + i;
+        if (a.positions && (i == 0 || !a.one_axis) && s_axis[pair] != axis) {      // neighbouring pairs are of one axis mostly
+          axis = s_axis[pair];
+          const int64_t place = row + axis * a.pa;
+          p = a.pos64 ? static_cast<const int64_t*>(a.positions)[place] : static_cast<const int32_t*>(a.positions)[place];
+        }
+        sincos_turn(static_cast<uint32_t>(static_cast<uint64_t>(p) * s_turns[pair] >> 32), sn[i], cs[i]);      // modulo one turn
+        cs[i] *= a.amplitude;
+        sn[i] *= a.inverse ? -a.amplitude : a.amplitude;
       }
-      if (kP == 1) {
-        dst[unit * 2] = static_cast<uint16_t>(w[0]);
-        dst[unit * 2 + 1] = static_cast<uint16_t>(w[0] >> 16);
-      } else {
-        copy_out<4 * kP>(dst + unit * 2 * kP, w);
-      }
-    } else {
-      constexpr int kW = kP > 1 ? kP / 2 : 1;
-      uint32_t u[kW], v[kW];
-      copy_in<2 * kP>(u, src + unit * kP);
-      copy_in<2 * kP>(v, src + a.half + unit * kP);
+    }
 #pragma unroll
-      for (int i = 0; i < kW; ++i) {
-        const float2 fu = widen<kBf16>(u[i]), fv = widen<kBf16>(v[i]);
-        const float c1 = kP > 1 ? cs[(2 * i + 1) % kP] : 0.0f, s1 = kP > 1 ? sn[(2 * i + 1) % kP] : 0.0f;
-        u[i] = pack2(fmaf(fu.x, cs[2 * i], -fv.x * sn[2 * i]), fmaf(fu.y, c1, -fv.y * s1), kType);
-        v[i] = pack2(fmaf(fv.x, cs[2 * i], fu.x * sn[2 * i]), fmaf(fv.y, c1, fu.y * s1), kType);
+    for (int j = 0; j < kBatch; ++j) {
+      if (h0 + j * a.lanes_h >= a.heads) continue;
+      uint16_t* dst = target(h0 + j * a.lanes_h) + at;
+      if (kP == 1) {
+        const float2 f = widen<kBf16>(u[j][0] | v[j][0] << 16);
+        const uint32_t w = pack2(fmaf(f.x, cs[0], -f.y * sn[0]), fmaf(f.y, cs[0], f.x * sn[0]), kType);
+        u[j][0] = w & 0xFFFFu;
+        v[j][0] = w >> 16;
+      } else if (kInterleaved) {
+#pragma unroll
+        for (int i = 0; i < kP; ++i) {
+          uint32_t& w = i < kW ? u[j][i % kW] : v[j][i % kW];
+          const float2 f = widen<kBf16>(w);
+          w = pack2(fmaf(f.x, cs[i], -f.y * sn[i]), fmaf(f.y, cs[i], f.x * sn[i]), kType);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kW; ++i) {
+          const float2 fu = widen<kBf16>(u[j][i]), fv = widen<kBf16>(v[j][i]);
+          const float2 c = make_float2(cs[2 * i], cs[(2 * i + 1) % kP]), s = make_float2(sn[2 * i], sn[(2 * i + 1) % kP]);
+          const float2 x = __ffma2_rn(fu, c, __fmul2_rn(fv, make_float2(-s.x, -s.y))), y = __ffma2_rn(fv, c, __fmul2_rn(fu, s));
+          u[j][i] = pack2(x.x, x.y, kType);
+          v[j][i] = pack2(y.x, y.y, kType);
+        }
       }
-      copy_out<2 * kP>(dst + unit * kP, u);
-      copy_out<2 * kP>(dst + a.half + unit * kP, v);
+      copy_out<2 * kP>(dst, u[j]);
+      copy_out<2 * kP>(dst + apart, v[j]);
     }
   }
 }
@@ -208,8 +267,8 @@ int apply(const hy3d_rotary_side* sides, int n_sides, int dtype, int64_t batch, 
   int pairs = 8;
   for (; pairs > 1; pairs >>= 1) {
     if (a.half % pairs || tail % (2 * pairs)) continue;
-    // half: 2 * pairs bytes at multiples of that; interleaved, and the copied rest: 4 * pairs bytes, as 16-byte vectors at most
-    const int el = (interleaved || tail) ? 2 * pairs : pairs, align = el < 8 ? el : 8;
+    // 2 * pairs bytes at multiples of that; the copied rest: 4 * pairs bytes, as 16-byte vectors at most
+    const int el = tail ? 2 * pairs : pairs, align = el < 8 ? el : 8;
     uint64_t all = 0;
     for (int i = 0; i < n_sides; ++i) {
       const hy3d_rotary_side& s = sides[i];
@@ -222,13 +281,13 @@ int apply(const hy3d_rotary_side* sides, int n_sides, int dtype, int64_t batch, 
     if ((all & (align - 1)) == 0 && (!tail || rot % align == 0)) break;
   }
   a.units = a.half / pairs;
-  a.units_all = a.units + (tail + 2 * pairs - 1) / (2 * pairs);
+  a.tail_units = (tail + 2 * pairs - 1) / (2 * pairs);
   const int rc = device_ok();
   if (rc != HY3D_OK) return rc;
-  // Heads of a thread: up to 8 share its sines and cosines; fewer where there are too few tokens to fill the SMs.
+  // Heads of a thread: up to 8 share its sines and cosines; fewer where that leaves an SM less than 1024 threads.
   const int sms = device_sm_count() > 0 ? device_sm_count() : 148;
   int per = 8;
-  while (per > 1 && a.tokens * a.units_all * ((a.heads + per - 1) / per) < static_cast<int64_t>(sms) * 2048) per >>= 1;
+  while (per > 1 && a.tokens * a.units * ((a.heads + per - 1) / per) < static_cast<int64_t>(sms) * 1024) per >>= 1;
   a.lanes_h = (a.heads + per - 1) / per;
   a.positions = positions;
   a.pos64 = pos64 != 0;
@@ -238,15 +297,20 @@ int apply(const hy3d_rotary_side* sides, int n_sides, int dtype, int64_t batch, 
   a.offset = offset;
   a.amplitude = amplitude;
   a.inverse = inverse != 0;
+  a.one_axis = 1;
   for (int i = 0; i < a.half; ++i) {
     a.turns[i] = turns[i];
     a.axis[i] = axis[i];
+    if (axis[i]) a.one_axis = 0;
   }
-  const int64_t per_token = static_cast<int64_t>(a.lanes_h) * a.units_all;
-  if (per_token > 0x7FFFFFFF || a.tokens > (int64_t{0x7FFFFFFF} * kThreads) / per_token) return HY3D_ERR_SHAPE;
-  a.small = a.tokens * per_token <= 0xFFFFFFFFll - kThreads;
+  const int64_t per_token = static_cast<int64_t>(a.lanes_h) * a.units, per_tail = static_cast<int64_t>(a.lanes_h) * a.tail_units;
+  const int64_t most = per_token > per_tail ? per_token : per_tail;
+  if (most > 0x3FFFFFFF || a.tokens > (int64_t{0x3FFFFFFF} * kThreads) / most) return HY3D_ERR_SHAPE;
+  a.small = a.tokens * most <= 0xFFFFFFFFll - kThreads;
+  a.turn_blocks = static_cast<uint32_t>((a.tokens * per_token + kThreads - 1) / kThreads);
+  const uint32_t copy_blocks = static_cast<uint32_t>((a.tokens * per_tail + kThreads - 1) / kThreads);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((a.tokens * per_token + kThreads - 1) / kThreads));
+  cfg.gridDim = dim3(a.turn_blocks + copy_blocks);
   cfg.blockDim = dim3(kThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1] = {pdl_attribute()};
