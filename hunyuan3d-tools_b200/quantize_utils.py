@@ -657,7 +657,8 @@ class Int4Linear(nn.Module):
     @torch.no_grad()
     def from_codes(codes, scale, zero=None, bias=None) -> "Int4Linear":
         """From codes (N,K) of 0..15, scales (N, K/group) in fp16 or bf16 and zero points of the same shape (whole numbers
-        0..15; 8 without them), as other quantisers produce them; bias (N) or None."""
+        0..15; 8 without them), as other quantisers produce them; bias (N) or None.  A scale may be a sixteenth of its
+        type's largest number at most, so that every weight ``scale * (code - zero)`` is a number of that type too."""
         if codes.dim() != 2 or codes.is_floating_point() or scale.dim() != 2 or scale.shape[0] != codes.shape[0] \
                 or scale.shape[1] < 1 or codes.shape[1] % scale.shape[1]:
             raise RuntimeError("Int4Linear.from_codes takes whole codes (N, K) and scales (N, K / group), "
@@ -667,6 +668,9 @@ class Int4Linear(nn.Module):
         for name, t in (("codes", codes), ("zero", zero)):
             if t is not None and t.numel() and (int(t.min()) < 0 or int(t.max()) > 15):
                 raise RuntimeError(f"Int4Linear.from_codes: {name} must lie between 0 and 15")
+        if scale.numel() and scale.is_floating_point() \
+                and not bool((scale.detach().float().abs() <= torch.finfo(scale.dtype).max / 16).all()):
+            raise RuntimeError("Int4Linear.from_codes: a scale is not finite or above a sixteenth of its type's largest number")
         n, k = codes.shape
         if bias is not None and tuple(bias.shape) != (n,):
             raise RuntimeError(f"Int4Linear.from_codes: bias must have {n} entries, got {tuple(bias.shape)}")
@@ -707,7 +711,8 @@ class Int4Linear(nn.Module):
 
     @staticmethod
     def concat(layers) -> "Int4Linear":
-        """One layer computing ``[l0(x) | l1(x) | ...]``; every output column keeps its bits."""
+        """One layer computing ``[l0(x) | l1(x) | ...]``; every output column keeps its weights.  (A sum's order
+        follows the layer's size, so its last bits may change.)"""
         layers = list(layers)
         first = layers[0]
         for l in layers:

@@ -198,11 +198,15 @@ int hy3d_rotary(const hy3d_rotary_side* sides, int n_sides, int dtype, int64_t b
  * with fp32 sums of exact products and one rounding to x's type.  x: (M,K) f16 / bf16, row pitch ldx (a multiple of 8).
  * w: codes 0..15 in tiles of 16 rows x 64 columns, [N/16][K/64][lane][4 words]: lane 4g + t holds rows g and g + 8; words 0
  * and 2 are row g's, words 1 and 3 row g + 8's.  The eight columns of words 0 and 1 are 4t .. 4t+3 and 16 + 4t .. 16 + 4t+3,
- * those of words 2 and 3 32 more; nibble j < 4 of a word is its column 2j, nibble 4 + j its column 2j + 1.  scale: f16 / bf16 [N/16][K/group][16], place 2g for row g and 2g + 1 for row g + 8.  zero: the
- * same places, a byte 0..15 each, or NULL for 8 throughout.  group: 32, or a multiple of 64; divides K.  bias (N) or NULL.
+ * those of words 2 and 3 32 more; nibble j < 4 of a word is its column 2j, nibble 4 + j its column 2j + 1.
+ * scale: f16 / bf16 [N/16][K/group][16], place 2g for row g and 2g + 1 for row g + 8; finite, and scale * 15 within the range
+ * of its type.  zero: the same places, a byte 0..15 each, or NULL for 8 throughout.  group: 32, or a multiple of 64; divides
+ * K.  bias (N) or NULL.
  * Epilogues as for the int8 GEMMs (HY3D_EPI_GEGLU: rows interleaved in blocks of 16, N / 2 columns out), GELU in its exact
  * form.  out: (M, N or N / 2) of x's type.  Requires K % 64 == 0, K <= 32768, N % 16 == 0 (% 32 GEGLU), 16-byte aligned x
  * rows, w, scale and zero, 8-byte aligned out.  No workspace.  No counterpart in the reference.
+ * Two kernels, which sum in different orders; shape and types decide, never the values, so equal calls give equal bits.  A row
+ * of x with a NaN or an infinity gives values that are not finite, and leaves the other rows as they are.
  */
 int hy3d_linear_w4(const void* x, int x_dtype, int64_t ldx, const void* w, const void* scale, int scale_dtype, const void* zero,
                    int64_t group, const void* bias, int bias_dtype, void* out, int64_t M, int64_t N, int64_t K, int epilogue,

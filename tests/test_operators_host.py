@@ -107,6 +107,25 @@ def test_int4_refusals(qu):
         layer(qu.QuantizedActivation(codes, scale, (16, 64), torch.float16))
 
 
+@pytest.mark.parametrize("dt,most", [(torch.float16, 4094.0), (torch.bfloat16, 2.1e37)])
+def test_int4_scales_leave_every_weight_in_range(qu, dt, most):
+    """A sixteenth of the largest number: 15 times that is finite, in a scale's own type."""
+    codes = torch.full((16, 64), 15)
+    zero = torch.zeros(16, 1, dtype=torch.uint8)
+    layer = qu.Int4Linear.from_codes(codes, torch.full((16, 1), most).to(dt), zero)
+    assert torch.isfinite(layer.dequantize_weight().to(dt)).all()
+    for bad in (most * 1.02, -most * 1.02, float("inf"), float("nan")):
+        scale = torch.ones(16, 1, dtype=dt)
+        scale[3, 0] = bad
+        with pytest.raises(RuntimeError, match="scale"):
+            qu.Int4Linear.from_codes(codes, scale, zero)
+    wide = nn.Linear(64, 16, bias=False).to(dt)
+    with torch.no_grad():
+        wide.weight[2, 5] = most * 7.5
+    with pytest.raises(RuntimeError, match="scale"):
+        qu.Int4Linear.from_linear(wide)
+
+
 def test_int4_model_surgery(qu):
     torch.manual_seed(3)
     net = nn.Sequential(nn.Linear(128, 256), nn.Sequential(nn.Linear(256, 64), nn.Linear(256, 200)), nn.Linear(256, 256))
