@@ -293,11 +293,14 @@ gemm_w4_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ CUtenso
   }
   __syncwarp();
   tc_fence_before_sync();
-  if (a.ks > 1) cluster_sync_all(); else __syncthreads();
+  __syncthreads();
+  // Before the cluster's barrier: a CTA that has tensor memory never waits for one that may be waiting for some.
   if (warp == kUnpackWarps) {
     tc_fence_after_sync();
     tmem_dealloc_1cta(tmem, static_cast<uint32_t>(a.tmem_cols));
   }
+  __syncwarp();
+  if (a.ks > 1) cluster_sync_all();
   const bool geglu = a.epilogue == HY3D_EPI_GEGLU;
   const int n_out = geglu ? a.N >> 1 : a.N;
   // A lane has four neighbouring rows, or with a gate the values of two outputs: two rows and the two 16 behind them.

@@ -87,7 +87,6 @@ __device__ __forceinline__ float2 scale_pair(uint32_t w, bool bf16) {
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
-
 __device__ __forceinline__ void bulk_prefetch_l2(const void* src, uint32_t bytes) {
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
 }
@@ -99,6 +98,7 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kPending>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory"); }
+
 // Few tokens (8 at most): bound by the stream of codes and, next to it, by the integer instructions that unpack them.  One
 // CTA per SM.  The activations of its tokens lie in shared memory whole; 2^lg_wk warps share a unit of kR blocks of 16
 // rows, each with a range of K, and take `trips` units one after the other without a pause, through rings of their own in
