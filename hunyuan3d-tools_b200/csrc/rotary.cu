@@ -8,10 +8,11 @@
 // no table of cosines to build, to keep or to outgrow.  The angle's top two bits are its quadrant, and the rest is small
 // enough for the Taylor polynomials of sine and cosine.
 //
-// Bound by HBM: 4 bytes of traffic per value (32768 tokens of 40 heads of 128: 106.8 us, 6.3 TB/s; 8 x 1 tokens: 2.6 us).
+// Bound by HBM: 4 bytes of traffic per value (32768 tokens of 40 heads of 128: 107 us, 6.3 TB/s; 8 x 1 tokens: 2.6 us).
 // A thread has the sines and cosines of 8 pairs and turns those of up to 8 heads with them, loads of four heads in flight at
-// a time: one head after the other with sincospif took 146 and 3.4.  With three axes (2 x 6144 tokens of 20 heads of 64: 15.9,
-// 4.0 TB/s) a thread waits for its positions before its sines, and has fewer heads to use them for.
+// a time: one head after the other with sincospif took 146 and 3.4.  Where few heads share the sines the instructions count
+// as much (2 x 6144 tokens over three axes, 20 heads of 64: 13.9 us, 4.5 TB/s, a thousand instructions per warp of 5 heads;
+// with each head's addresses from its strides instead of additions 15.9).
 #include "common.cuh"
 
 namespace hy3d {
@@ -27,6 +28,7 @@ struct Side {                     // queries or keys
   const uint16_t* src;
   uint16_t* dst;
   int64_t sb, sn, sh, db, dn, dh; // strides of batch, token and head, elements
+  int heads, lanes;               // threads of a token that share a unit's heads, lanes apart
 };
 struct Args {
   Side side[2];
@@ -34,10 +36,9 @@ struct Args {
   int64_t pb, pn, pa, offset;
   int64_t tokens;                 // batch * n
   uint32_t n;                     // tokens of a sequence
-  int heads0, heads;              // of the first side, of both
   int units, tail_units;          // of a head: turned, and only copied
   uint32_t turn_blocks;           // blocks that turn; the others copy
-  int lanes_h;                    // threads of a token that share a unit's heads
+  int lanes;                      // of both sides
   int half, dim;                  // rotated pairs; dimensions of a head
   float amplitude;
   uint8_t pos64, inverse, small, one_axis;
@@ -99,11 +100,11 @@ __device__ __forceinline__ void sincos_turn(uint32_t phase, float& s, float& c) 
 
 constexpr int kBatch = 4;         // heads whose loads are in flight together
 
-// The first blocks turn: a thread has one unit of one token and walks over that token's heads, lanes_h apart.
-// Neighbouring threads have neighbouring units, then neighbouring heads.  The blocks behind them copy the dimensions that
+// The first blocks turn: a thread has one unit of one token and walks over that token's heads of one side, by additions to
+// two addresses.  Neighbouring threads have neighbouring units, then neighbouring heads, the keys' behind the queries'.  The blocks behind them copy the dimensions that
 // are not turned, in the same order.
 template <bool kBf16, bool kInterleaved, int kP>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 3)
 rotary_kernel(const __grid_constant__ Args a) {
   __shared__ uint64_t s_turns[kMaxPairs];
   __shared__ uint8_t s_axis[kMaxPairs];
@@ -119,7 +120,7 @@ rotary_kernel(const __grid_constant__ Args a) {
   }
   const int units = copies ? a.tail_units : a.units;
   const int64_t id = static_cast<int64_t>(copies ? blockIdx.x - a.turn_blocks : blockIdx.x) * kThreads + threadIdx.x;
-  const uint32_t per_token = static_cast<uint32_t>(a.lanes_h * units);
+  const uint32_t per_token = static_cast<uint32_t>(a.lanes * units);
   int64_t token, b;
   if (a.small) {                  // a 64-bit division costs as much as the sines
     token = static_cast<uint32_t>(id) / per_token;
@@ -130,34 +131,35 @@ rotary_kernel(const __grid_constant__ Args a) {
   }
   if (token >= a.tokens) return;
   const uint32_t rest = static_cast<uint32_t>(id - token * per_token);
-  const int first_head = rest / units, unit = rest - first_head * units;
+  const int lane = static_cast<int>(rest / static_cast<uint32_t>(units)), unit = static_cast<int>(rest) - lane * units;
   const uint32_t n = static_cast<uint32_t>(token - b * a.n);
+  const bool second = lane >= a.side[0].lanes;
+  const Side& side = a.side[second];
+  const int first_head = second ? lane - a.side[0].lanes : lane, lanes = side.lanes;
+  int left = (side.heads - first_head + lanes - 1) / lanes;      // heads to go
+  const int64_t step_src = lanes * side.sh, step_dst = lanes * side.dh;
+  const uint16_t* src = side.src + b * side.sb + n * side.sn + first_head * side.sh;
+  uint16_t* dst = side.dst + b * side.db + n * side.dn + first_head * side.dh;
   pdl_wait();
-  auto source = [&](int h) {
-    const Side& s = a.side[h >= a.heads0];
-    return s.src + b * s.sb + n * s.sn + (h >= a.heads0 ? h - a.heads0 : h) * s.sh;
-  };
-  auto target = [&](int h) {
-    const Side& s = a.side[h >= a.heads0];
-    return s.dst + b * s.db + n * s.dn + (h >= a.heads0 ? h - a.heads0 : h) * s.dh;
-  };
 
   if (copies) {
     const int at = 2 * a.half + unit * 2 * kP;
-    for (int h0 = first_head; h0 < a.heads; h0 += kBatch * a.lanes_h) {
+    src += at;
+    dst += at;
+    for (; left > 0; left -= kBatch) {
       if (kP == 1) {
-        for (int h = h0; h < a.heads && h < h0 + kBatch * a.lanes_h; h += a.lanes_h) {
-          target(h)[at] = source(h)[at];
-          if (at + 1 < a.dim) target(h)[at + 1] = source(h)[at + 1];
+        for (int j = 0; j < kBatch && j < left; ++j, src += step_src, dst += step_dst) {
+          dst[0] = src[0];
+          if (at + 1 < a.dim) dst[1] = src[1];
         }
       } else {
         uint32_t w[kBatch][kP];
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j)
-          if (h0 + j * a.lanes_h < a.heads) copy_in<4 * kP>(w[j], source(h0 + j * a.lanes_h) + at);
+        for (int j = 0; j < kBatch; ++j, src += step_src)
+          if (j < left) copy_in<4 * kP>(w[j], src);
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j)
-          if (h0 + j * a.lanes_h < a.heads) copy_out<4 * kP>(target(h0 + j * a.lanes_h) + at, w[j]);
+        for (int j = 0; j < kBatch; ++j, dst += step_dst)
+          if (j < left) copy_out<4 * kP>(dst, w[j]);
       }
     }
     return;
@@ -166,17 +168,19 @@ rotary_kernel(const __grid_constant__ Args a) {
   float cs[kP], sn[kP];
   const int at = kInterleaved && kP == 1 ? 2 * unit : unit * kP, apart = kInterleaved && kP == 1 ? 1 : a.half;
   constexpr int kW = kP > 1 ? kP / 2 : 1;
-  for (int h0 = first_head; h0 < a.heads; h0 += kBatch * a.lanes_h) {
+  src += at;
+  dst += at;
+  for (bool first = true; left > 0; left -= kBatch, first = false) {
     uint32_t u[kBatch][kW], v[kBatch][kW];         // the vectors at the two places
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      if (h0 + j * a.lanes_h >= a.heads) continue;
-      const uint16_t* src = source(h0 + j * a.lanes_h) + at;
+    for (int j = 0; j < kBatch; ++j, src += step_src) {
+      if (j >= left) continue;
       copy_in<2 * kP>(u[j], src);
       copy_in<2 * kP>(v[j], src + apart);
     }
-    if (h0 == first_head) {                        // while the first loads are under way
+    if (first) {                        // while the first loads are under way
       const int64_t row = b * a.pb + n * a.pn;
+      const float sine_amplitude = a.inverse ? -a.amplitude : a.amplitude;
       int64_t p = a.offset + n;
       int axis = -1;
 #pragma unroll
@@ -189,13 +193,12 @@ rotary_kernel(const __grid_constant__ Args a) {
         }
         sincos_turn(static_cast<uint32_t>(static_cast<uint64_t>(p) * s_turns[pair] >> 32), sn[i], cs[i]);      // modulo one turn
         cs[i] *= a.amplitude;
-        sn[i] *= a.inverse ? -a.amplitude : a.amplitude;
+        sn[i] *= sine_amplitude;
       }
     }
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      if (h0 + j * a.lanes_h >= a.heads) continue;
-      uint16_t* dst = target(h0 + j * a.lanes_h) + at;
+    for (int j = 0; j < kBatch; ++j, dst += step_dst) {
+      if (j >= left) continue;
       if (kP == 1) {
         const float2 f = widen<kBf16>(u[j][0] | v[j][0] << 16);
         const uint32_t w = pack2(fmaf(f.x, cs[0], -f.y * sn[0]), fmaf(f.y, cs[0], f.x * sn[0]), kType);
@@ -256,12 +259,10 @@ int apply(const hy3d_rotary_side* sides, int n_sides, int dtype, int64_t batch, 
     if (s.heads < 0 || s.heads > 1 << 20) return HY3D_ERR_SHAPE;
     if (s.heads > 0 && (!s.src || !s.dst)) return HY3D_ERR_ARG;
     if ((reinterpret_cast<uintptr_t>(s.src) | reinterpret_cast<uintptr_t>(s.dst)) & 1) return HY3D_ERR_SHAPE;
-    a.side[i] = {static_cast<const uint16_t*>(s.src), static_cast<uint16_t*>(s.dst), s.src_b, s.src_n, s.src_h, s.dst_b, s.dst_n, s.dst_h};
-    a.heads += s.heads;
-    if (i == 0) a.heads0 = s.heads;
+    a.side[i] = {static_cast<const uint16_t*>(s.src), static_cast<uint16_t*>(s.dst), s.src_b, s.src_n, s.src_h, s.dst_b, s.dst_n, s.dst_h, s.heads, 0};
     in_place = in_place && (s.heads == 0 || s.src == s.dst);
   }
-  if (a.heads == 0) return HY3D_OK;
+  if (a.side[0].heads + a.side[1].heads == 0) return HY3D_OK;
   // Pairs of a unit: the most whose vectors are whole and aligned everywhere.
   const int tail = in_place ? 0 : dim - rot;
   int pairs = 8;
@@ -286,9 +287,11 @@ int apply(const hy3d_rotary_side* sides, int n_sides, int dtype, int64_t batch, 
   if (rc != HY3D_OK) return rc;
   // Heads of a thread: up to 8 share its sines and cosines; fewer where that leaves an SM less than 1024 threads.
   const int sms = device_sm_count() > 0 ? device_sm_count() : 148;
-  int per = 8;
-  while (per > 1 && a.tokens * a.units * ((a.heads + per - 1) / per) < static_cast<int64_t>(sms) * 1024) per >>= 1;
-  a.lanes_h = (a.heads + per - 1) / per;
+  for (int per = 8; per > 0; per >>= 1) {
+    a.lanes = 0;
+    for (Side& side : a.side) a.lanes += side.lanes = (side.heads + per - 1) / per;
+    if (a.tokens * a.units * a.lanes >= static_cast<int64_t>(sms) * 1024) break;
+  }
   a.positions = positions;
   a.pos64 = pos64 != 0;
   a.pb = pb;
@@ -303,7 +306,7 @@ int apply(const hy3d_rotary_side* sides, int n_sides, int dtype, int64_t batch, 
     a.axis[i] = axis[i];
     if (axis[i]) a.one_axis = 0;
   }
-  const int64_t per_token = static_cast<int64_t>(a.lanes_h) * a.units, per_tail = static_cast<int64_t>(a.lanes_h) * a.tail_units;
+  const int64_t per_token = static_cast<int64_t>(a.lanes) * a.units, per_tail = static_cast<int64_t>(a.lanes) * a.tail_units;
   const int64_t most = per_token > per_tail ? per_token : per_tail;
   if (most > 0x3FFFFFFF || a.tokens > (int64_t{0x3FFFFFFF} * kThreads) / most) return HY3D_ERR_SHAPE;
   a.small = a.tokens * most <= 0xFFFFFFFFll - kThreads;
