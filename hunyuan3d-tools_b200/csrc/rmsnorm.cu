@@ -57,34 +57,38 @@ struct Args {
   int K, lg, g_dtype;
 };
 
-// Eight of gamma's values as pairs; `raw` are the 16-bit ones, loaded earlier.
+// Eight of gamma's values as pairs.  kOwn: of the activations' type, `raw` loaded earlier.
+template <bool kBf16, bool kOwn>
 __device__ __forceinline__ void gamma_pairs(const Args& a, int vec, const uint4& raw, float2 (&g)[4]) {
-  if (!a.gamma) {
+  float f[8];
+  if (kOwn) {
+    unpack8<kBf16>(raw, f);
+  } else if (!a.gamma) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) g[j] = make_float2(1.0f, 1.0f);
+    for (int j = 0; j < 8; ++j) f[j] = 1.0f;
   } else if (a.g_dtype == HY3D_F32) {
     const float4* p = reinterpret_cast<const float4*>(a.gamma) + 2 * vec;
     const float4 u = __ldg(p), v = __ldg(p + 1);
-    g[0] = make_float2(u.x, u.y); g[1] = make_float2(u.z, u.w);
-    g[2] = make_float2(v.x, v.y); g[3] = make_float2(v.z, v.w);
+    f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w;
+    f[4] = v.x; f[5] = v.y; f[6] = v.z; f[7] = v.w;
   } else {
-    float f[8];
-    if (a.g_dtype == HY3D_BF16) unpack8<true>(raw, f); else unpack8<false>(raw, f);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) g[j] = make_float2(f[2 * j], f[2 * j + 1]);
+    unpack8<!kBf16>(__ldg(reinterpret_cast<const uint4*>(a.gamma) + vec), f);
   }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) g[j] = make_float2(f[2 * j], f[2 * j + 1]);
 }
 
 // 2^lg threads share a row, each with up to kV 16-byte vectors that stay in registers between the statistics and the
 // output.  A block holds blockDim >> lg rows; threads past the last row compute it too and store nothing.
-// Bound by HBM with a residual (12288 x 640 to 16 bits 9.3 us, 6.7 TB/s; to codes 10.7, 5.1; 8192 x 8192 to 16 bits 81.3,
-// 6.6).  Without one, to codes, by the chain of load, two reductions and store with too few rows in flight (3855 x 1536 7.9 us,
-// 2.2 TB/s; 49152 x 320 13.9, 3.4); blocks per SM follow from the registers kV needs, none of which may spill: with three
-// blocks for every kV those two took 8.6 and 14.8.  (A grid-stride loop that requests the next row ahead of the current
-// one's work spilled: 12288 x 640 10.8 -> 13.2.)
-// gamma's 16-bit values are requested with the row's, not after its statistics, where there are registers for both: one row
-// of 4096 3.2 -> 2.5 us.
-template <bool kBf16, int kV, bool kAdd, bool kCodes, bool kWide>
+// Bound by HBM with a residual (12288 x 640 to 16 bits 8.6 us, 7.4 TB/s, part of it still in L2; to codes 9.9, 5.6; 8192 x 8192
+// to 16 bits 80.3, 6.7).  Without one, to codes, by instructions and the chain of load, two reductions and store (3855 x 1536
+// 7.2 us, 2.5 TB/s; 49152 x 320 13.0, 3.6).  Blocks per SM follow from the registers kV needs, none of which may spill: with
+// three blocks for every kV those two took 8 and 6 % more.  (A grid-stride loop that requests the next row ahead of the current
+// one's work spilled: 12288 x 640 to codes 10.8 -> 13.2.)
+// kOwn: gamma is of the activations' type, and its values are requested with the row's, not after its statistics, where there
+// are registers for both.  With its type looked up for every vector one row of 4096 took 2.5 us instead of 2.1, 3855 x 1536
+// 7.9, 12288 x 640 to codes 10.7 and 4096 x 4096 23.0 instead of 19.4.
+template <bool kBf16, int kV, bool kAdd, bool kCodes, bool kWide, bool kOwn>
 __global__ void __launch_bounds__(kWide ? 512 : kThreads, kWide ? 2 : kV == 1 ? 6 : kV == 2 ? 5 : kV == 3 ? 4 : 3)
 rmsnorm_kernel(const __grid_constant__ Args a) {
   __shared__ float s_part[2][16];
@@ -114,9 +118,9 @@ rmsnorm_kernel(const __grid_constant__ Args a) {
       if (live && sub + i * G < nvec) dst[i * G] = v[i];
     }
   }
-  constexpr bool kEarly = !kCodes || kV <= (kWide ? 3 : 4);
+  constexpr bool kEarly = kOwn && (!kCodes || kV <= (kWide ? 3 : 4));
   uint4 graw[kV];
-  if (kEarly && a.gamma && a.g_dtype != HY3D_F32)
+  if (kEarly)
 #pragma unroll
     for (int i = 0; i < kV; ++i)
       graw[i] = sub + i * G < nvec ? __ldg(reinterpret_cast<const uint4*>(a.gamma) + sub + i * G) : make_uint4(0, 0, 0, 0);
@@ -147,8 +151,8 @@ rmsnorm_kernel(const __grid_constant__ Args a) {
   for (int i = 0; i < kV; ++i) {
     if (sub + i * G < nvec) {
       float2 g[4];
-      if (!kEarly && a.gamma && a.g_dtype != HY3D_F32) graw[i] = __ldg(reinterpret_cast<const uint4*>(a.gamma) + sub + i * G);
-      gamma_pairs(a, sub + i * G, graw[i], g);
+      if (kOwn && !kEarly) graw[i] = __ldg(reinterpret_cast<const uint4*>(a.gamma) + sub + i * G);
+      gamma_pairs<kBf16, kOwn>(a, sub + i * G, graw[i], g);
       float f[8];
       unpack8<kBf16>(v[i], f);
       uint32_t w[4];
@@ -194,9 +198,9 @@ int launch(const Args& in, cudaStream_t stream) {
   Args a = in;
   const int nvec = a.K >> 3;
   // Threads per row: the fewest (a power of two, eight where the row has as many vectors, so that a load touches whole 128-byte
-  // lines: 30000 x 64 5.6 -> 3.8 us) that hold it with 4 vectors each; eight threads take 5.  More vectors a thread and fewer
-  // threads save reductions and barriers (at most 3 vectors: 5000 x 2048 to codes 11.9 -> 14.1 us, 49152 x 320 13.9 -> 16.4),
-  // fewer vectors leave registers for more blocks on an SM (5: 12288 x 640 to 16 bits 9.3 -> 10.1).  By K alone: the number
+  // lines: 30000 x 64 a third less) that hold it with 4 vectors each; eight threads take 5.  More vectors a thread and fewer
+  // threads save reductions and barriers (at most 3 vectors: 5000 x 2048 to codes and 49152 x 320 18 % more),
+  // fewer vectors leave registers for more blocks on an SM (5: 12288 x 640 to 16 bits 8 % more).  By K alone: the number
   // of threads fixes the order of the row's sum, so a row's result does not depend on how many others there are.
   a.lg = 0;
   while ((a.lg < 3 && (1 << a.lg) < nvec) || ((nvec + (1 << a.lg) - 1) >> a.lg) > (a.lg == 3 ? 5 : 4)) ++a.lg;
@@ -213,14 +217,17 @@ int launch(const Args& in, cudaStream_t stream) {
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   using KernelFn = void (*)(const Args);
-#define HY3D_RMS(V, W)                                                                      \
-  {{rmsnorm_kernel<kBf16, V, false, false, W>, rmsnorm_kernel<kBf16, V, false, true, W>},   \
-   {rmsnorm_kernel<kBf16, V, true, false, W>, rmsnorm_kernel<kBf16, V, true, true, W>}}
-  static const KernelFn kernels[5][2][2] = {HY3D_RMS(1, false), HY3D_RMS(2, false), HY3D_RMS(3, false), HY3D_RMS(4, false),
-                                            HY3D_RMS(5, false)};
-  static const KernelFn wide[2][2][2] = {HY3D_RMS(3, true), HY3D_RMS(4, true)};      // 512 threads: K from 8200 on, 3 or 4 vectors each
+#define HY3D_RMS2(V, A, C, W) {rmsnorm_kernel<kBf16, V, A, C, W, false>, rmsnorm_kernel<kBf16, V, A, C, W, true>}
+#define HY3D_RMS(V, W)                                                    \
+  {{HY3D_RMS2(V, false, false, W), HY3D_RMS2(V, false, true, W)},         \
+   {HY3D_RMS2(V, true, false, W), HY3D_RMS2(V, true, true, W)}}
+  static const KernelFn kernels[5][2][2][2] = {HY3D_RMS(1, false), HY3D_RMS(2, false), HY3D_RMS(3, false), HY3D_RMS(4, false),
+                                               HY3D_RMS(5, false)};
+  static const KernelFn wide[2][2][2][2] = {HY3D_RMS(3, true), HY3D_RMS(4, true)};      // 512 threads: K from 8200 on
 #undef HY3D_RMS
-  const KernelFn kernel = a.lg > 8 ? wide[v - 3][a.add ? 1 : 0][a.q ? 1 : 0] : kernels[v - 1][a.add ? 1 : 0][a.q ? 1 : 0];
+#undef HY3D_RMS2
+  const int own = a.gamma && a.g_dtype == (kBf16 ? HY3D_BF16 : HY3D_F16) ? 1 : 0;
+  const KernelFn kernel = (a.lg > 8 ? wide[v - 3] : kernels[v - 1])[a.add ? 1 : 0][a.q ? 1 : 0][own];
   if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) {
     cudaGetLastError();
     return HY3D_ERR_CUDA;
