@@ -8,10 +8,10 @@
 // no table of cosines to build, to keep or to outgrow.  The angle's top two bits are its quadrant, and the rest is small
 // enough for the Taylor polynomials of sine and cosine.
 //
-// Bound by HBM: 4 bytes of traffic per value (32768 tokens of 40 heads of 128: 107 us, 6.3 TB/s; 8 x 1 tokens: 2.6 us).
+// Bound by HBM: 4 bytes of traffic per value (32768 tokens of 40 heads of 128: 105 us, 6.4 TB/s; 8 x 1 tokens: 2.0 us).
 // A thread has the sines and cosines of 8 pairs and turns those of up to 8 heads with them, loads of four heads in flight at
 // a time: one head after the other with sincospif took 146 and 3.4.  Where few heads share the sines the instructions count
-// as much (2 x 6144 tokens over three axes, 20 heads of 64: 13.9 us, 4.5 TB/s, a thousand instructions per warp of 5 heads;
+// as much (2 x 6144 tokens over three axes, 20 heads of 64: 13.2 us, 4.8 TB/s, a thousand instructions per warp of 5 heads;
 // with each head's addresses from its strides instead of additions 15.9).
 #include "common.cuh"
 
@@ -21,7 +21,7 @@ int device_ok();
 namespace rotary {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kMaxPairs = 256;
 
 struct Side {                     // queries or keys
@@ -41,7 +41,7 @@ struct Args {
   int lanes;                      // of both sides
   int half, dim;                  // rotated pairs; dimensions of a head
   float amplitude;
-  uint8_t pos64, inverse, small, one_axis;
+  uint8_t pos64, inverse, small;
   uint8_t axis[kMaxPairs];
   uint64_t turns[kMaxPairs];
 };
@@ -103,18 +103,20 @@ constexpr int kBatch = 4;         // heads whose loads are in flight together
 // The first blocks turn: a thread has one unit of one token and walks over that token's heads of one side, by additions to
 // two addresses.  Neighbouring threads have neighbouring units, then neighbouring heads, the keys' behind the queries'.  The blocks behind them copy the dimensions that
 // are not turned, in the same order.
-template <bool kBf16, bool kInterleaved, int kP>
-__global__ void __launch_bounds__(kThreads, 3)
+// kAxes: pairs of several axes, each with a position of its own.  Five blocks an SM leave the registers for four heads without
+// spills (six: 107 us and 22.8 for 105 and 22.2); with several axes six are better all the same (13.2 us, five 14.9).
+template <bool kBf16, bool kInterleaved, int kP, bool kAxes>
+__global__ void __launch_bounds__(kThreads, kAxes ? 6 : 5)
 rotary_kernel(const __grid_constant__ Args a) {
   __shared__ uint64_t s_turns[kMaxPairs];
-  __shared__ uint8_t s_axis[kMaxPairs];
+  __shared__ uint8_t s_axis[kAxes ? kMaxPairs : 1];
   pdl_launch_dependents();
   constexpr int kType = kBf16 ? HY3D_BF16 : HY3D_F16;
   const bool copies = blockIdx.x >= a.turn_blocks;
   if (!copies) {                  // indexed by lane, the parameter itself would be read one address after the other
     for (int i = threadIdx.x; i < a.half; i += kThreads) {
       s_turns[i] = a.turns[i];
-      s_axis[i] = a.axis[i];
+      if (kAxes) s_axis[i] = a.axis[i];
     }
     __syncthreads();
   }
@@ -180,16 +182,18 @@ rotary_kernel(const __grid_constant__ Args a) {
     }
     if (first) {                        // while the first loads are under way
       const int64_t row = b * a.pb + n * a.pn;
+      auto position = [&](int64_t place) {
+        return a.pos64 ? static_cast<const int64_t*>(a.positions)[place] : static_cast<int64_t>(static_cast<const int32_t*>(a.positions)[place]);
+      };
       const float sine_amplitude = a.inverse ? -a.amplitude : a.amplitude;
-      int64_t p = a.offset + n;
+      int64_t p = !kAxes && a.positions ? position(row) : a.offset + n;
       int axis = -1;
 #pragma unroll
       for (int i = 0; i < kP; ++i) {
         const int pair = kInterleaved && kP > 1 ? unit * kW + i + (i < kW ? 0 : (a.half >> 1) - kW) : unit * kP + i;
-        if (a.positions && (i == 0 || !a.one_axis) && s_axis[pair] != axis) {      // neighbouring pairs are of one axis mostly
+        if (kAxes && s_axis[pair] != axis) {       // neighbouring pairs are of one axis mostly
           axis = s_axis[pair];
-          const int64_t place = row + axis * a.pa;
-          p = a.pos64 ? static_cast<const int64_t*>(a.positions)[place] : static_cast<const int32_t*>(a.positions)[place];
+          p = position(row + axis * a.pa);
         }
         sincos_turn(static_cast<uint32_t>(static_cast<uint64_t>(p) * s_turns[pair] >> 32), sn[i], cs[i]);      // modulo one turn
         cs[i] *= a.amplitude;
@@ -228,13 +232,13 @@ rotary_kernel(const __grid_constant__ Args a) {
 }
 
 using KernelFn = void (*)(const Args);
-template <bool kBf16, bool kInterleaved>
+template <bool kBf16, bool kInterleaved, bool kAxes>
 KernelFn kernel_of(int pairs) {
   switch (pairs) {
-    case 8: return rotary_kernel<kBf16, kInterleaved, 8>;
-    case 4: return rotary_kernel<kBf16, kInterleaved, 4>;
-    case 2: return rotary_kernel<kBf16, kInterleaved, 2>;
-    default: return rotary_kernel<kBf16, kInterleaved, 1>;
+    case 8: return rotary_kernel<kBf16, kInterleaved, 8, kAxes>;
+    case 4: return rotary_kernel<kBf16, kInterleaved, 4, kAxes>;
+    case 2: return rotary_kernel<kBf16, kInterleaved, 2, kAxes>;
+    default: return rotary_kernel<kBf16, kInterleaved, 1, kAxes>;
   }
 }
 
@@ -300,11 +304,11 @@ int apply(const hy3d_rotary_side* sides, int n_sides, int dtype, int64_t batch, 
   a.offset = offset;
   a.amplitude = amplitude;
   a.inverse = inverse != 0;
-  a.one_axis = 1;
+  bool many_axes = false;         // without positions every axis has the token's index
   for (int i = 0; i < a.half; ++i) {
     a.turns[i] = turns[i];
     a.axis[i] = axis[i];
-    if (axis[i]) a.one_axis = 0;
+    if (axis[i] && positions) many_axes = true;
   }
   const int64_t per_token = static_cast<int64_t>(a.lanes) * a.units, per_tail = static_cast<int64_t>(a.lanes) * a.tail_units;
   const int64_t most = per_token > per_tail ? per_token : per_tail;
@@ -319,8 +323,11 @@ int apply(const hy3d_rotary_side* sides, int n_sides, int dtype, int64_t batch, 
   cudaLaunchAttribute attr[1] = {pdl_attribute()};
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const KernelFn kernel = dtype == HY3D_BF16 ? (interleaved ? kernel_of<true, true>(pairs) : kernel_of<true, false>(pairs))
-                                             : (interleaved ? kernel_of<false, true>(pairs) : kernel_of<false, false>(pairs));
+  const KernelFn kernel =
+      many_axes ? (dtype == HY3D_BF16 ? (interleaved ? kernel_of<true, true, true>(pairs) : kernel_of<true, false, true>(pairs))
+                                      : (interleaved ? kernel_of<false, true, true>(pairs) : kernel_of<false, false, true>(pairs)))
+                : (dtype == HY3D_BF16 ? (interleaved ? kernel_of<true, true, false>(pairs) : kernel_of<true, false, false>(pairs))
+                                      : (interleaved ? kernel_of<false, true, false>(pairs) : kernel_of<false, false, false>(pairs)));
   if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) {
     cudaGetLastError();
     return HY3D_ERR_CUDA;
