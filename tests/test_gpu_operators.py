@@ -98,6 +98,38 @@ def test_int4_leading_dimensions_strides_and_scale_types(qu):
     _check_int4(layer, w, b, x, layer(x))
 
 
+@pytest.mark.parametrize("k,n,group,zeros,epilogue", [(576, 176, 32, True, "linear"), (2048, 288, 64, False, "geglu"),
+                                                      (32768, 48, 256, True, "gelu")])
+def test_int4_every_number_of_tokens_around_the_kernels_limits(qu, k, n, group, zeros, epilogue):
+    """8 tokens a pass of one kernel, 16 a column block of the other, 256 a CTA; rows of x taken out of a longer matrix."""
+    layer, w, b = _int4(qu, n, k, group, zeros, True, torch.float16, k, epilogue)
+    x = (torch.randn(520, k + 64, generator=_gen(n), device=DEV) * (2.0 if k < 32768 else 0.125)).half()[:, :k]
+    for m in (1, 7, 8, 9, 15, 16, 17, 24, 33, 63, 64, 65, 80, 255, 256, 257, 513):
+        _check_int4(layer, w, b, x[:m], layer(x[:m]))
+
+
+@pytest.mark.parametrize("dtype,size,values", [(torch.float16, 2.0 ** -21, 1000.0), (torch.float16, 4094.0, 2.0 ** -9),
+                                               (torch.bfloat16, 2.0 ** -126, 2.0 ** 20), (torch.bfloat16, 2.0 ** 60, 1.0)])
+def test_int4_scales_at_the_ends_of_their_type(qu, dtype, size, values):
+    """The two numbers of a weight are exact for subnormal scales and for the largest; activations of a size that keeps
+    products and results in range."""
+    g = _gen(8)
+    scale = (size * (torch.rand(176, 4, generator=g, device=DEV).double() * 0.9 + 0.1)).to(dtype)
+    codes = torch.randint(0, 16, (176, 256), generator=g, device=DEV)
+    zero = torch.randint(0, 16, (176, 4), generator=g, device=DEV)
+    layer = qu.Int4Linear.from_codes(codes, scale, zero)
+    w = (codes - zero.repeat_interleave(64, 1)).double() * scale.double().repeat_interleave(64, 1)
+    x = (torch.randn(100, 256, generator=g, device=DEV) * values).to(dtype)
+    for m in (3, 100):
+        _check_int4(layer, w, None, x[:m], layer(x[:m]))
+
+
+def test_int4_scales_of_another_type_for_many_rows(qu):
+    layer, w, b = _int4(qu, 112, 448, 64, True, True, torch.bfloat16, 9)
+    x = torch.randn(333, 448, generator=_gen(3), device=DEV).half()
+    _check_int4(layer, w, b, x, layer(x))
+
+
 def test_int4_infinities_and_nans_stay_in_their_rows(qu):
     layer, w, b = _int4(qu, 64, 256, 64, False, True, torch.bfloat16, 6)
     for m in (5, 40, 300):
