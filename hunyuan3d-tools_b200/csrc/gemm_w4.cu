@@ -377,11 +377,12 @@ TcFn tc_kernel_of(bool sub, bool plain) {
 TcPlan tc_plan(int64_t M, int64_t N, int64_t K) {
   TcPlan p = {16, 1, 1, INT64_MAX};
   const int64_t bx = (N + 127) / 128, tiles = K / 64, fewest = (M + 255) / 256;
+  int64_t at_once[9];
+  for (int ks = 1; ks <= 8; ++ks) at_once[ks] = resident_clusters(ks, 1) > 0 ? resident_clusters(ks, 1) : 128 / ks;
   for (int64_t ctas = fewest; ctas <= (M + 15) / 16 && ctas <= fewest + 15; ++ctas) {
     const int64_t t = ((M + ctas - 1) / ctas + 15) / 16 * 16, by = (M + t - 1) / t;
     for (int ks = 1; ks <= 8 && (ks == 1 || tiles >= 4 * ks); ++ks) {
-      const int64_t at_once = resident_clusters(ks, 1) > 0 ? resident_clusters(ks, 1) : 128 / ks;
-      const int64_t tile = 4 * t > 540 ? 4 * t : 540, waves = (bx * by + at_once - 1) / at_once;
+      const int64_t tile = 4 * t > 540 ? 4 * t : 540, waves = (bx * by + at_once[ks] - 1) / at_once[ks];
       const int64_t cycles = waves * ((tiles + ks - 1) / ks * tile + 6000 + 12 * t + (ks > 1 ? 1500 : 0));
       if (cycles < p.cycles) p = {static_cast<int>(t), ks, by, cycles};
     }
