@@ -227,9 +227,9 @@ class Attention(nn.Module):
                 k, v = self.to_k(context), self.to_v(context)
         q = q.view(b, n, self.heads, c // self.heads)
         k = k.view(b, m, self.heads, c // self.heads)
-        if self.rotary is not None:       # both are this call's own: turned where they lie
+        if self.rotary is not None:       # into new tensors: a hook may have kept the projections' outputs
             at = None if self.rotary_positions is None else self.rotary_positions[n]
-            q, k = self.rotary(q, k, at, inplace=True)
+            q, k = self.rotary(q, k, at)
         q, k = q.transpose(1, 2), k.transpose(1, 2)
         v = v.view(b, m, self.heads, c // self.heads).transpose(1, 2)
         o = F.scaled_dot_product_attention(q, k, v)

@@ -514,3 +514,16 @@ def test_unet_with_multiview_rotary_rmsnorms_and_four_bit_projections(qu, pkg):
     # normal weight, in the time path only; the int8 path adds 1 %
     assert float((loose.float() - turned.float()).norm() / turned.float().norm()) < 0.15
     assert float((fused.float() - loose.float()).norm() / loose.float().norm()) < 0.03
+
+
+def test_attention_leaves_the_projections_outputs_to_their_hooks(pkg):
+    """A hook on a projection keeps what the projection returned; the rotation writes to tensors of its own."""
+    un = importlib.import_module(PKG + ".unet")
+    attn = un.TransformerBlock(128, 2, 128, 2).attn_mv.to(DEV).bfloat16()
+    attn.rotary = importlib.import_module(PKG + ".rotary").RotaryPositions(64)
+    kept = []
+    attn.to_q.register_forward_hook(lambda m, a, y: kept.append(y))
+    x = torch.randn(1, 12, 128, generator=_gen(4), device=DEV).bfloat16()
+    with torch.no_grad():
+        attn(x)
+        assert torch.equal(kept[0], nn.functional.linear(x, attn.to_q.weight, attn.to_q.bias))
