@@ -92,7 +92,6 @@ gemm_w4_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ CUtenso
   const int b_bytes = a.tokens * 128, stage_bytes = 2 * b_bytes, n = end - first, pairs = (n + 1) >> 1;
   volatile int* abort_flag = &ctrl.abort_flag;
 
-  pdl_launch_dependents();
   if (warp == kUnpackWarps) {
     if (lane == 0) {
       for (int i = 0; i < a.stages; ++i) {
@@ -113,6 +112,9 @@ gemm_w4_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ CUtenso
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = ctrl.tmem, tmem_a = tmem + static_cast<uint32_t>(a.d_cols);
+  // Not before every CTA of the grid has its tensor memory: the next kernel takes its own and then waits for this one to
+  // end, so a CTA still without would wait for columns that are held until it is done.
+  pdl_launch_dependents();
 
   bool ok = true;
   if (warp < kUnpackWarps) {
@@ -422,6 +424,8 @@ int gemm(const void* x, int x_dtype, int64_t ldx, const void* w, const void* sca
   int smem = a.stages * stage_bytes + rings;
   if (smem < a.tokens * kSumPitch * 4) smem = a.tokens * kSumPitch * 4;
   smem += 1024;
+  // One CTA per SM: each takes all 512 columns of tensor memory, so a second could only wait for them.
+  if (smem < 120 * 1024) smem = 120 * 1024;
   CUtensorMap tm_x;
   int rc = encode_tmap_2d_u8(&tm_x, x, static_cast<uint64_t>(2 * K), static_cast<uint64_t>(M), static_cast<uint64_t>(2 * ldx), 128,
                              static_cast<uint32_t>(a.tokens), 128);
