@@ -32,6 +32,8 @@ __host__ __device__ constexpr int slot_bytes(int sub, bool plain) { return 512 +
 __host__ __device__ constexpr int ring_depth(int sub, bool plain) { return slot_bytes(sub, plain) <= 640 ? 8 : 5; }
 
 struct TcArgs {
+  const uint16_t* x;
+  int64_t ldx;
   const uint4* w;
   const uint32_t* scale;      // pairs (row g, row g + 8)
   const uint8_t* zero;        // the same, a byte each; or null
@@ -74,6 +76,64 @@ __host__ __device__ constexpr uint32_t make_idesc_f16(bool bf16, uint32_t m, uin
 }
 
 constexpr uint32_t kNegateA = 1u << 13;
+
+// The sum of one output as the definition has it, in order, up to the first NaN.
+template <bool kBf16>
+__device__ __noinline__ float sum_by_definition(const TcArgs& a, int token, int row) {
+  const int tiles = a.K >> 6, group = a.K / a.groups, half = row >> 3 & 1, g = row & 7;
+  const int64_t block = row >> 4;
+  const uint16_t* x = a.x + token * a.ldx;
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(a.w) + block * tiles * 128 + 16 * g + half;
+  float y = 0.0f;
+  for (int k = 0; k < a.K && y == y; k += 32) {
+    const int64_t at = (block * a.groups + k / group) * 16 + 2 * g + half;
+    const uint16_t bits = reinterpret_cast<const uint16_t*>(a.scale)[at];
+    const float scale = kBf16 ? __uint_as_float(static_cast<uint32_t>(bits) << 16) : __half2float(__ushort_as_half(bits));
+    const int zero = a.zero ? a.zero[at] : 8;
+    float sum = 0.0f;
+    for (int t = 0; t < 4; ++t) {      // columns 4t .. 4t + 3 and 16 + 4t .. 16 + 4t + 3
+      const uint32_t codes = w[(k >> 6) * 128 + 4 * t + (k >> 4 & 2)];
+      for (int i = 0; i < 8; ++i) {
+        const int code = static_cast<int>(codes >> (4 * (i >> 1) + 16 * (i & 1)) & 15u);
+        const uint16_t v = x[k + 4 * t + 16 * (i >> 2) + (i & 3)];
+        sum = fmaf(kBf16 ? __uint_as_float(static_cast<uint32_t>(v) << 16) : __half2float(__ushort_as_half(v)),
+                   static_cast<float>(code - zero), sum);
+      }
+    }
+    y = fmaf(scale, sum, y);
+  }
+  return y;
+}
+
+// A lane's outputs of a token, packed: from the sums of rows `row` and `row + 1` and of those `gates` behind.
+template <bool kBf16>
+__device__ __forceinline__ uint2 outputs_of(int epilogue, const float (&y)[4]) {
+  constexpr int kType = kBf16 ? HY3D_BF16 : HY3D_F16;
+  if (epilogue == HY3D_EPI_GEGLU) {
+    const float2 gate = gelu_phi2(make_float2(y[2], y[3]));
+    return make_uint2(pack2(y[0] * gate.x, y[1] * gate.y, kType), 0u);
+  }
+  float2 u = make_float2(y[0], y[1]), v = make_float2(y[2], y[3]);
+  if (epilogue == HY3D_EPI_GELU) {
+    u = gelu_phi2(u);
+    v = gelu_phi2(v);
+  }
+  return make_uint2(pack2(u.x, u.y, kType), pack2(v.x, v.y, kType));
+}
+
+// A running maximum of packed pairs, in which a NaN stays.
+template <bool kBf16>
+__device__ __forceinline__ uint32_t max_or_nan(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if (kBf16) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <bool kBf16>
+__device__ __forceinline__ bool has_nan(uint32_t w) {
+  constexpr uint32_t kInf = kBf16 ? 0x7F80u : 0x7C00u;
+  return (w & 0x7FFFu) > kInf || (w >> 16 & 0x7FFFu) > kInf;
+}
 
 // kPlain: no zero points.
 template <bool kBf16, int kSub, bool kPlain>
@@ -314,7 +374,7 @@ gemm_w4_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ CUtenso
 #pragma unroll
     for (int i = 0; i < 4; ++i) bias[i] = load_scalar(a.bias, a.bias_dtype, row + (i & 1) + (i >> 1) * gates);
   }
-  constexpr int kType = kBf16 ? HY3D_BF16 : HY3D_F16;
+  uint32_t seen = 0;
   const uint32_t at0 = smem_u32(s_sum + local);
 #pragma unroll 1
   for (int tok = rank + a.ks * warp; tok < a.tokens; tok += a.ks * static_cast<int>(blockDim.x >> 5)) {
@@ -346,17 +406,30 @@ gemm_w4_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ CUtenso
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] += bias[i];
+    const uint2 w = outputs_of<kBf16>(a.epilogue, y);
     uint16_t* out = a.out + static_cast<int64_t>(tok0 + tok) * n_out + col;
+    seen = max_or_nan<kBf16>(seen, w.x);
     if (geglu) {
-      const float2 gate = gelu_phi2(make_float2(y[2], y[3]));
-      *reinterpret_cast<uint32_t*>(out) = pack2(y[0] * gate.x, y[1] * gate.y, kType);
+      *reinterpret_cast<uint32_t*>(out) = w.x;
     } else {
-      float2 u = make_float2(y[0], y[1]), v = make_float2(y[2], y[3]);
-      if (a.epilogue == HY3D_EPI_GELU) {
-        u = gelu_phi2(u);
-        v = gelu_phi2(v);
-      }
-      *reinterpret_cast<uint2*>(out) = make_uint2(pack2(u.x, u.y, kType), pack2(v.x, v.y, kType));
+      *reinterpret_cast<uint2*>(out) = w;
+      seen = max_or_nan<kBf16>(seen, w.y);
+    }
+  }
+  // Two numbers a weight cannot give the sum where an activation is infinite: lo is 0 for most weights, and infinity times that
+  // is NaN, where infinity times the weight keeps its sign.  A lane's outputs that are NaN are made once more, from the
+  // definition.  (The look for them costs 1 to 2 %: 924 x 1024 -> 2560 10.7 us, without it 10.5.)
+  if (has_nan<kBf16>(seen)) {
+    for (int tok = rank + a.ks * warp; tok < a.tokens && tok0 + tok < a.M; tok += a.ks * static_cast<int>(blockDim.x >> 5)) {
+      uint16_t* out = a.out + static_cast<int64_t>(tok0 + tok) * n_out + col;
+      uint32_t* out2 = reinterpret_cast<uint32_t*>(out);
+      if (!has_nan<kBf16>(out2[0]) && (geglu || !has_nan<kBf16>(out2[1]))) continue;
+      float y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = sum_by_definition<kBf16>(a, tok0 + tok, row + (i & 1) + (i >> 1) * gates) + bias[i];
+      const uint2 w = outputs_of<kBf16>(a.epilogue, y);
+      out2[0] = w.x;
+      if (!geglu) out2[1] = w.y;
     }
   }
   __syncwarp();
@@ -396,6 +469,8 @@ TcPlan tc_plan(int64_t M, int64_t N, int64_t K) {
 int gemm(const void* x, int x_dtype, int64_t ldx, const void* w, const void* scale, const void* zero, int64_t group, const void* bias,
          int bias_dtype, void* out, int64_t M, int64_t N, int64_t K, int epilogue, const TcPlan& plan, cudaStream_t stream) {
   TcArgs a;
+  a.x = static_cast<const uint16_t*>(x);
+  a.ldx = ldx;
   a.w = static_cast<const uint4*>(w);
   a.scale = static_cast<const uint32_t*>(scale);
   a.zero = static_cast<const uint8_t*>(zero);

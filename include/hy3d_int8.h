@@ -205,8 +205,8 @@ int hy3d_rotary(const hy3d_rotary_side* sides, int n_sides, int dtype, int64_t b
  * Epilogues as for the int8 GEMMs (HY3D_EPI_GEGLU: rows interleaved in blocks of 16, N / 2 columns out), GELU in its exact
  * form.  out: (M, N or N / 2) of x's type.  Requires K % 64 == 0, K <= 32768, N % 16 == 0 (% 32 GEGLU), 16-byte aligned x
  * rows, w, scale and zero, 8-byte aligned out.  No workspace.  No counterpart in the reference.
- * Two kernels, which sum in different orders; shape and types decide, never the values, so equal calls give equal bits.  A row
- * of x with a NaN or an infinity gives values that are not finite, and leaves the other rows as they are.
+ * Two kernels, which sum in different orders; shape and types decide, never the values, so equal calls give equal bits.  An
+ * infinity or a NaN in x gives what the sum above gives for it in either kernel, and leaves the other rows as they are.
  */
 int hy3d_linear_w4(const void* x, int x_dtype, int64_t ldx, const void* w, const void* scale, int scale_dtype, const void* zero,
                    int64_t group, const void* bias, int bias_dtype, void* out, int64_t M, int64_t N, int64_t K, int epilogue,
