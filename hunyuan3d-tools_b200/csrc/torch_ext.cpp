@@ -13,6 +13,8 @@
 #include <Python.h>
 #include <dlfcn.h>
 
+#include <algorithm>
+
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/Context.h>
 #include <ATen/autocast_mode.h>
@@ -823,8 +825,6 @@ struct Turned {
     if (d == 4) { b = v.size(0); sb = v.stride(0); }
     t = &v;
   }
-  int64_t row(int64_t dim) const { return (h - 1) * sh + dim; }                  // elements from a token's first to its last
-  int64_t sequence(int64_t dim) const { return (n - 1) * sn + row(dim); }
   // Whether no two elements lie in the same place: each stride steps over all that the smaller ones reach.
   bool separate(int64_t dim) const {
     int64_t size[3] = {b, n, h}, stride[3] = {sb, sn, sh};
@@ -840,22 +840,37 @@ struct Turned {
     return true;
   }
 };
-// Whether two tensors that are turned in place share no element: apart altogether, or side by side in every sequence or
-// in every token of equal steps (a stacked projection).
+// Whether two tensors that are turned in place, each of separate elements, share none: apart altogether, or with the same
+// steps in their outer dimensions and side by side between two places there (a stacked projection: in every
+// token, sequence or head).  Tensors that meet nowhere but step differently are not told apart.
 bool apart(const Turned& a, const Turned& b, int64_t dim) {
   if (a.t->numel() == 0 || b.t->numel() == 0) return true;
-  const int64_t size = a.t->element_size();
-  const char *pa = static_cast<const char*>(a.t->const_data_ptr()), *pb = static_cast<const char*>(b.t->const_data_ptr());
-  const int64_t gap = (pb - pa) / size;
-  auto beside = [&](int64_t ea, int64_t eb, int64_t step) {       // intervals of ea and eb elements, repeated every `step`
-    return gap >= 0 ? gap >= ea && gap + eb <= step : -gap >= eb && -gap + ea <= step;
-  };
-  constexpr int64_t kNever = int64_t{1} << 62;
-  const int64_t whole_a = (a.b - 1) * a.sb + a.sequence(dim), whole_b = (b.b - 1) * b.sb + b.sequence(dim);
-  if (beside(whole_a, whole_b, kNever)) return true;
-  if (a.sb == b.sb && a.sb > 0 && beside(a.sequence(dim), b.sequence(dim), a.sb)) return true;
-  const bool batches_apart = a.b == 1 || (a.sb == b.sb && a.sb >= (a.n - 1) * a.sn + a.sn && a.sn == b.sn);
-  return a.sn == b.sn && a.sn > 0 && batches_apart && beside(a.row(dim), b.row(dim), a.sn);
+  struct Dim { int64_t na, nb, sa, sb; } d[3] = {{a.b, b.b, a.sb, b.sb}, {a.n, b.n, a.sn, b.sn}, {a.h, b.h, a.sh, b.sh}};
+  for (Dim& x : d) {              // a dimension of one has no step of its own
+    if (x.na == 1) x.sa = x.nb == 1 ? 0 : x.sb;
+    if (x.nb == 1) x.sb = x.sa;
+  }
+  std::sort(d, d + 3, [](const Dim& x, const Dim& y) { return x.sa > y.sa; });
+  const int64_t gap = (static_cast<const char*>(b.t->const_data_ptr()) - static_cast<const char*>(a.t->const_data_ptr())) /
+                      static_cast<int64_t>(a.t->element_size());
+  // The least distance of two different places in the outer dimensions: a step of the last, or one of the others less all
+  // steps of the last.
+  int64_t step = int64_t{1} << 62;
+  for (int outer = 0; outer <= 3; ++outer) {
+    int64_t reach_a = dim, reach_b = dim;
+    for (int i = outer; i < 3; ++i) {
+      reach_a += (d[i].na - 1) * d[i].sa;
+      reach_b += (d[i].nb - 1) * d[i].sb;
+    }
+    if (gap >= 0 ? gap >= reach_a && gap + reach_b <= step : -gap >= reach_b && -gap + reach_a <= step) return true;
+    if (outer == 3) break;
+    const Dim& x = d[outer];
+    const int64_t most = x.na > x.nb ? x.na : x.nb;
+    if (x.sa != x.sb) return false;
+    if (most > 1) step = std::min(x.sa, step - (most - 1) * x.sa);
+    if (step <= 0) return false;
+  }
+  return false;
 }
 
 // rotary(plan, q, k | None, positions | None, offset, inverse, inplace) -> q | (q, k) | None; `plan` is RotaryPositions' own:

@@ -86,7 +86,8 @@ class RotaryPositions:
     def __call__(self, q, k=None, positions=None, offset=0, inverse=False, inplace=False):
         """q (B, N, H, D) or (N, H, D), k likewise with its own number of heads, or None; any strides with adjacent head
         dimensions (a (B, H, N, D) tensor is passed transposed).  Returns q, or (q, k): new contiguous tensors, or with
-        ``inplace`` the same ones turned.  ``positions``: int64 or int32, (N) or (B, N), with several axes
+        ``inplace`` the same ones turned (side by side in whatever a projection returned: in each token, sequence or head).
+        ``positions``: int64 or int32, (N) or (B, N), with several axes
         (N, axes) or (B, N, axes); ``offset`` + 0, 1, 2 ... when there are none (one axis only).  ``inverse`` turns back:
         the inverse of the turn, and its transpose where the amplitude is 1."""
         y = (_qu._NATIVE or _qu._load_native()).rotary(self._plan, q, k, positions, offset, inverse, inplace)
@@ -128,7 +129,8 @@ class RotaryPositions:
         elif len(self.axes) > 1:
             raise RuntimeError("rotary: positions are needed where there are several axes")
         if inplace:
-            raise RuntimeError("rotary: in place, no two elements of q and k may share memory")
+            raise RuntimeError("rotary: in place, no two elements of q and k may share memory, and where they interleave, "
+                               "their outer dimensions must have the same strides")
         raise RuntimeError("rotary: a tensor subclass, a layout other than strided, or an argument of another type")
 
     def __repr__(self):

@@ -34,3 +34,46 @@ def test_int4_infinite_activations_give_what_the_definition_gives(qu, dtype, m, 
     assert torch.equal(~y.isfinite(), bad) and bool(ref[0].isinf().any()) and bool(ref[0].isnan().any())
     assert torch.equal(y[bad].isnan(), ref[bad].isnan())
     assert torch.equal(y[bad & ~ref.isnan()].double(), ref[bad & ~ref.isnan()])
+
+
+def test_rotary_in_place_wherever_queries_and_keys_share_no_element(rotary):
+    """Side by side in every token of a sequence-first tensor, in every head of an interleaved one, and in strided slices of
+    those; refused where a single element is shared."""
+    r, b, n, h, d = rotary.RotaryPositions(64), 3, 7, 4, 64
+    g = _gen(21)
+
+    def check(whole, q, k):
+        other = torch.ones_like(whole, dtype=torch.bool)
+        for t in (q, k):
+            other.as_strided(t.shape, t.stride(), t.storage_offset()).fill_(False)
+        rest = whole[other].clone()
+        want = r(q, k)
+        got = r(q, k, inplace=True)
+        assert got[0] is q and torch.equal(q, want[0]) and torch.equal(k, want[1])
+        assert torch.equal(whole[other], rest)
+
+    whole = torch.randn(n, b, 3 * h * d, generator=g, device=DEV).half()              # sequence first
+    q, k, _ = (t.view(n, b, h, d).transpose(0, 1) for t in whole.split(h * d, dim=-1))
+    check(whole, q, k)
+    whole = torch.randn(n, b, (h + 2) * d, generator=g, device=DEV).half()            # the same with one key head
+    check(whole, whole[..., :h * d].view(n, b, h, d).transpose(0, 1), whole[..., h * d:(h + 1) * d].view(n, b, 1, d).transpose(0, 1))
+    whole = torch.randn(b, n, h, 3, d, generator=g, device=DEV).half()                # q, k and v of each head together
+    check(whole, whole[..., 0, :], whole[..., 1, :])
+    check(whole, whole[:, ::2, :, 2], whole[:, ::2, :, 0])
+    check(whole[0], whole[0, ..., 1, :], whole[0, ..., 0, :])
+    whole = torch.randn(n, b, h, 3, d, generator=g, device=DEV).half()                # and sequence first
+    check(whole, whole[..., 0, :].transpose(0, 1), whole[..., 2, :].transpose(0, 1))
+    whole = torch.randn(b, n, 2 * h, d, generator=g, device=DEV).half()               # heads in turn
+    check(whole, whole[:, :, 0::2], whole[:, :, 1::2])
+    whole = torch.randn(b, 2 * n, h, d, generator=g, device=DEV).half()               # tokens in turn
+    check(whole, whole[:, 0::2], whole[:, 1::2])
+
+    flat = torch.randn(b * n * h * d * 4, generator=g, device=DEV).half()
+    size = (b, n, h, d)
+    q = flat.as_strided(size, (n * h * 2 * d, h * 2 * d, 2 * d, 1), 0)
+    for at in (d - 1, d + 1, 2 * d * h + d // 2, 2 * d):          # the last element; the next head's; inside a token; a head further
+        k = flat.as_strided(size, q.stride(), at)
+        with pytest.raises(RuntimeError, match="share memory"):
+            r(q, k, inplace=True)
+    with pytest.raises(RuntimeError, match="share memory"):       # other steps: nothing is known of where they meet
+        r(q, flat.as_strided(size, (n * h * 3 * d, h * 3 * d, 3 * d, 1), d), inplace=True)
