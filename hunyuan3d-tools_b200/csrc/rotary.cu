@@ -2,9 +2,10 @@
 //     (u, v) -> (u cos a - v sin a, v cos a + u sin a) * amplitude,    a = position[axis(i)] * w_i
 // for the queries and the keys of one call, out of place or in place, in either direction (the inverse turns by -a).
 //
-// The angle is exact at any position: w_i comes as a 64-bit fraction of a turn, 2^64 w_i / (2 pi), so the product with
-// the integer position is the angle modulo one turn by itself -- the integer product wraps where the circle does.  Its
-// error is position * 2^-65 turns; the fp32 product position * w_i would be off by 0.06 radians at a million.  There is
+// The angle loses next to nothing at far positions: w_i comes as a 64-bit fraction of a turn, 2^64 w_i / (2 pi) to the
+// nearest, so the product with the integer position is the angle modulo one turn by itself -- the integer product wraps
+// where the circle does.  Its error is position * 2^-65 turns (4e-10 radians at 2^31, 2e-7 at 2^40), and 2^-32 turns, 1.5e-9
+// radians, for the low half that is left out; the fp32 product position * w_i would be off by 0.06 at a million.  There is
 // no table of cosines to build, to keep or to outgrow.  The angle's top two bits are its quadrant, and the rest is small
 // enough for the Taylor polynomials of sine and cosine.
 //
@@ -79,7 +80,7 @@ __device__ __forceinline__ float2 widen(uint32_t w) {
 }
 
 // Sine and cosine of a 64-bit fraction of a turn, whose top 32 bits are given: x = angle past the nearest quarter turn,
-// |x| <= pi / 4, where the next terms are below 2e-9 (sine, relative) and 3e-8 (cosine).
+// |x| <= pi / 4, where the next terms are below 2.3e-9 (sine, relative) and 3e-8 (cosine).
 __device__ __forceinline__ void sincos_turn(uint32_t phase, float& s, float& c) {
   const uint32_t shifted = phase + 0x20000000u, quadrant = shifted >> 30;
   const float x = static_cast<float>(static_cast<int32_t>(shifted & 0x3FFFFFFFu) - 0x20000000) * 1.4629180792671596e-9f;     // 2 pi / 2^32

@@ -6,12 +6,17 @@ they lie (``inplace``), or into new tensors.  ``unet.Attention`` calls it when i
 """
 from __future__ import annotations
 
+import decimal
 import math
 import struct
 
 import torch
 
 from . import quantize_utils as _qu
+
+# Frequencies are made in 60 digits: a 64-bit fraction of a turn has more than a double keeps.
+_DIGITS = decimal.Context(prec=60)
+_TWO_PI = decimal.Decimal("6.28318530717958647692528676655900576839433879875021164194988918")
 
 
 class RotaryPositions:
@@ -48,16 +53,22 @@ class RotaryPositions:
             raise RuntimeError(f"base must be positive and amplitude finite, got {base} and {amplitude}")
         self.head_dim, self.rotary_dim, self.base, self.interleaved = head_dim, rotary_dim, float(base), bool(interleaved)
         self.axes, self.scaling, self.amplitude = axes, dict(scaling) if scaling else None, float(amplitude)
-        self.frequencies = [w for d in axes for w in self._axis_frequencies(d)]
-        # a fraction of a turn per unit of position, in 2^-64ths (modulo a whole turn)
-        turns = [int(math.ldexp(math.fmod(w / (2.0 * math.pi), 1.0), 64)) for w in self.frequencies]
+        with decimal.localcontext(_DIGITS):
+            exact = [w for d in axes for w in self._axis_frequencies(d)]
+            # a fraction of a turn per unit of position, in 2^-64ths (modulo a whole turn), to the nearest
+            turns = [w / _TWO_PI for w in exact]
+            turns = [int(((t - t.to_integral_value(decimal.ROUND_FLOOR)) * 2 ** 64).to_integral_value()) % 2 ** 64 for t in turns]
+        self.frequencies = [float(w) for w in exact]
+        if not all(math.isfinite(w) for w in self.frequencies):
+            raise RuntimeError(f"rotary frequencies out of range: base {base}, scaling {scaling}")
         self._turns = struct.pack(f"={len(turns)}Q", *turns)
         self._axis = bytes(a for a, d in enumerate(axes) for _ in range(d // 2))
         self._plan = (self.head_dim, self.rotary_dim, len(axes), self.interleaved, self._turns, self._axis, self.amplitude)
 
     def _axis_frequencies(self, d):
+        """Radians per unit of position of each pair of an axis, as decimals."""
         s = self.scaling or {"kind": "none"}
-        kind, base = s.get("kind"), self.base
+        kind, base = s.get("kind"), decimal.Decimal(self.base)
         allowed = {"none": set(), "linear": {"factor"}, "ntk": {"factor"},
                    "by_parts": {"factor", "original_length", "slow", "fast"}}
         if kind not in allowed:
@@ -65,22 +76,27 @@ class RotaryPositions:
         if set(s) - {"kind"} - allowed[kind]:
             raise RuntimeError(f"rotary scaling {kind!r} does not take {sorted(set(s) - {'kind'} - allowed[kind])}")
         if kind == "none":
-            factor = 1.0
+            factor = decimal.Decimal(1)
         else:
             factor = float(s.get("factor", 0.0))
             if not (factor > 0 and math.isfinite(factor)):
                 raise RuntimeError(f"rotary scaling needs a positive factor, got {s.get('factor')}")
+            factor = decimal.Decimal(factor)
         if kind == "ntk" and d > 2:
-            base *= factor ** (d / (d - 2))
-        w = [base ** (-2.0 * i / d) for i in range(d // 2)]
+            base *= factor ** (decimal.Decimal(d) / (d - 2))
+        ratio = base ** (decimal.Decimal(-2) / d)
+        w = [decimal.Decimal(1)]
+        while len(w) < d // 2:
+            w.append(w[-1] * ratio)
         if kind == "linear":
             return [v / factor for v in w]
         if kind == "by_parts":
             length, slow, fast = s.get("original_length", 0), s.get("slow", 1.0), s.get("fast", 4.0)
             if not (length > 0 and fast > slow):
                 raise RuntimeError("rotary scaling 'by_parts' needs original_length > 0 and fast > slow")
-            keep = [min(1.0, max(0.0, (length * v / (2.0 * math.pi) - slow) / (fast - slow))) for v in w]
-            return [v * k + v / factor * (1.0 - k) for v, k in zip(w, keep)]
+            length, slow, fast = (decimal.Decimal(float(v)) for v in (length, slow, fast))
+            keep = [min(decimal.Decimal(1), max(decimal.Decimal(0), (length * v / _TWO_PI - slow) / (fast - slow))) for v in w]
+            return [v * k + v / factor * (1 - k) for v, k in zip(w, keep)]
         return w
 
     def __call__(self, q, k=None, positions=None, offset=0, inverse=False, inplace=False):

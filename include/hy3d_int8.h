@@ -175,7 +175,8 @@ int hy3d_dequantize_rows(const int8_t* q, const float* scale, int64_t M, int64_t
  * interleaved -- and pair i turns by the angle position[axis[i]] * turns[i] / 2^64 of a full turn (inverse: by minus that):
  *   (u, v) -> (u cos a - v sin a, v cos a + u sin a) * amplitude, computed in fp32 and rounded once
  * The other dimensions are copied.  turns and axis are HOST arrays of rot / 2 entries; the product with the position is
- * taken modulo 2^64, which is modulo one turn, so the angle is exact at any position.
+ * taken modulo 2^64, which is modulo one turn, so far positions lose only what the fraction was rounded by: with the nearest
+ * one, position * 2^-65 turns, and 2^-32 turns of the product.
  * One or two sides (queries, keys) of `batch` sequences of n tokens, each with its own number of heads and strides (in
  * elements; the head's dimensions are adjacent).  dst == src with the same strides turns in place; other overlaps are the
  * caller's error.  positions: int64 or int32 device array, element of (b, token, axis) at b * pb + token * pn + axis * pa,

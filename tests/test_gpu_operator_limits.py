@@ -1,11 +1,13 @@
 """GPU: the 4-bit layers, the RMSNorms and the rotary positions at their limits, against their definitions in 64 bits."""
+import decimal
 import importlib
 import math
 
 import pytest
 import torch
 
-from test_gpu_operators import DEV, _gen
+from test_gpu_operators import DEV, HALF, TINY, _gen, _within
+from test_operator_limits_host import _frequencies_of_many_digits, _pi
 
 pytestmark = pytest.mark.gpu
 PKG = "hunyuan3d-tools_b200"
@@ -77,3 +79,31 @@ def test_rotary_in_place_wherever_queries_and_keys_share_no_element(rotary):
             r(q, k, inplace=True)
     with pytest.raises(RuntimeError, match="share memory"):       # other steps: nothing is known of where they meet
         r(q, flat.as_strided(size, (n * h * 3 * d, h * 3 * d, 3 * d, 1), d), inplace=True)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("base,scaling", [(10000.0, None), (500000.0, {"kind": "ntk", "factor": 4.0}),
+                                          (10000.0, {"kind": "by_parts", "factor": 8.0, "original_length": 8192})])
+def test_rotary_far_positions_against_angles_of_many_digits(rotary, interleaved, base, scaling):
+    """The angles from the formula in 60 digits, not from the plan's own fractions.  Those are within 2^-65 of a turn, so an
+    angle is off by position 2^-65 2 pi, on top of the 4e-7 of its evaluation in 32 bits."""
+    r = rotary.RotaryPositions(64, base=base, scaling=scaling, interleaved=interleaved)
+    far = [0, 1, 131071, 2 ** 31 - 1, 2 ** 31 + 5, 2 ** 36 + 1, 2 ** 40 + 3, -2 ** 40, -1, 999999]
+    angle, pi = [], _pi()
+    with decimal.localcontext() as ctx:
+        ctx.prec = 60
+        for p in far:
+            for w in _frequencies_of_many_digits(64, base, scaling):
+                angle.append(float(p * w % (2 * pi)))
+    angle = torch.tensor(angle, dtype=torch.float64, device=DEV).view(len(far), 1, 32)
+    q = torch.randn(len(far), 4, 64, generator=_gen(31), device=DEV).half()
+    got = r(q, None, torch.tensor(far, device=DEV))
+    t = q.double()
+    u, v = (t[..., 0::2], t[..., 1::2]) if interleaved else (t[..., :32], t[..., 32:])
+    c, s = angle.cos(), angle.sin()
+    y, z = u * c - v * s, v * c + u * s
+    off = 4e-7 + torch.tensor([abs(p) * 2.0 ** -65 * 2 * math.pi for p in far], dtype=torch.float64, device=DEV)[:, None, None]
+    tol = (u.abs() + v.abs()) * off
+    join = (lambda a, b: torch.stack([a, b], -1).flatten(-2)) if interleaved else (lambda a, b: torch.cat([a, b], -1))
+    ref, tol = join(y, z), join(tol, tol)
+    _within(got, ref, tol + HALF[torch.float16] * (ref.abs() + tol) + TINY[torch.float16])

@@ -1,5 +1,6 @@
 """CPU: rules that the 4-bit layers, the RMSNorms and the rotary positions keep at their limits."""
 import ctypes
+import decimal
 import importlib
 import os
 import re
@@ -14,6 +15,11 @@ PKG = "hunyuan3d-tools_b200"
 @pytest.fixture(scope="module")
 def lib(build_mod):
     return importlib.import_module(PKG + ".csrc._binding").configure(build_mod.load_library())
+
+
+@pytest.fixture(scope="module")
+def rotary():
+    return importlib.import_module(PKG + ".rotary")
 
 
 # ---- order of the kernels' first steps ------------------------------------------------------
@@ -35,3 +41,50 @@ def test_tensor_memory_is_taken_before_the_next_kernel_may_start(build_mod):
             assert min(starts) > max(takes), f"{name}: the next kernel may start before tensor memory is taken"
             assert "__syncthreads()" in body[max(takes):min(starts)], f"{name}: no barrier behind the allocation"
     assert found == 5
+
+
+# ---- angles in 60 digits, apart from the plan ------------------------------------------------
+def _pi():
+    """Machin: pi / 4 = 4 arctan(1 / 5) - arctan(1 / 239)."""
+    with decimal.localcontext() as ctx:
+        ctx.prec = 70
+
+        def arctan_of_one_over(n):
+            term = total = decimal.Decimal(1) / n
+            i, sign = 1, 1
+            while abs(term) > decimal.Decimal(10) ** -68:
+                term, i, sign = term / (n * n), i + 2, -sign
+                total += sign * term / i
+            return total
+        return 4 * (4 * arctan_of_one_over(5) - arctan_of_one_over(239))
+
+
+def _frequencies_of_many_digits(d, base, scaling):
+    base, scaling = decimal.Decimal(base), scaling or {}
+    factor = decimal.Decimal(scaling.get("factor", 1))
+    if scaling.get("kind") == "ntk":
+        base *= ((decimal.Decimal(d) / (d - 2)) * factor.ln()).exp()
+    out = []
+    for i in range(d // 2):
+        w = (-(decimal.Decimal(2 * i) / d) * base.ln()).exp()
+        if scaling.get("kind") == "linear":
+            w /= factor
+        elif scaling.get("kind") == "by_parts":      # whole below 1 turn in the original length, none from 4 on
+            keep = min(decimal.Decimal(1), max(decimal.Decimal(0), (scaling["original_length"] * w / (2 * _pi()) - 1) / 3))
+            w = w * keep + w / factor * (1 - keep)
+        out.append(w)
+    return out
+
+
+@pytest.mark.parametrize("d,base,scaling", [(64, 10000.0, None), (128, 500000.0, None), (96, 10000.0, {"kind": "linear", "factor": 3.0}),
+                                            (64, 10000.0, {"kind": "ntk", "factor": 4.0}),
+                                            (128, 10000.0, {"kind": "by_parts", "factor": 8.0, "original_length": 8192}), (2, 7.5, None)])
+def test_rotary_fractions_are_the_nearest(rotary, d, base, scaling):
+    """Half of the last of 64 bits, and 1e-6 of it for the 60 digits that both are made in."""
+    r = rotary.RotaryPositions(d, base=base, scaling=scaling)
+    with decimal.localcontext() as ctx:
+        ctx.prec = 70
+        exact = [w / (2 * _pi()) * 2 ** 64 for w in _frequencies_of_many_digits(d, base, scaling)]
+        for t, e, w in zip(memoryview(r._turns).cast("Q"), exact, r.frequencies, strict=True):
+            assert abs(t - e) <= decimal.Decimal("0.500001")
+            assert w == float(e / 2 ** 64 * (2 * _pi()))
