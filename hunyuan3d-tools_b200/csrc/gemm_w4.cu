@@ -450,7 +450,7 @@ TcFn tc_kernel_of(bool sub, bool plain) {
 // run at the same time, not in SMs: 15 of eight, and with 16 (148 SMs have room for their
 // CTAs) 200 x 8192 -> 2048 took 41.9 us instead of 18.1, 66 x 4096 -> 1024 14.1 instead of 9.4.
 TcPlan tc_plan(int64_t M, int64_t N, int64_t K) {
-  TcPlan p = {16, 1, 1, INT64_MAX};
+  TcPlan p = {16, 1, INT64_MAX};
   const int64_t bx = (N + 127) / 128, tiles = K / 64, fewest = (M + 255) / 256;
   int64_t at_once[9];
   for (int ks = 1; ks <= 8; ++ks) at_once[ks] = resident_clusters(ks, 1) > 0 ? resident_clusters(ks, 1) : 128 / ks;
@@ -459,7 +459,7 @@ TcPlan tc_plan(int64_t M, int64_t N, int64_t K) {
     for (int ks = 1; ks <= 8 && (ks == 1 || tiles >= 4 * ks); ++ks) {
       const int64_t tile = 4 * t > 540 ? 4 * t : 540, waves = (bx * by + at_once[ks] - 1) / at_once[ks];
       const int64_t cycles = waves * ((tiles + ks - 1) / ks * tile + 6000 + 12 * t + (ks > 1 ? 1500 : 0));
-      if (cycles < p.cycles) p = {static_cast<int>(t), ks, by, cycles};
+      if (cycles < p.cycles) p = {static_cast<int>(t), ks, cycles};
     }
   }
   return p;
@@ -469,25 +469,21 @@ TcPlan tc_plan(int64_t M, int64_t N, int64_t K) {
 int gemm(const void* x, int x_dtype, int64_t ldx, const void* w, const void* scale, const void* zero, int64_t group, const void* bias,
          int bias_dtype, void* out, int64_t M, int64_t N, int64_t K, int epilogue, const TcPlan& plan, cudaStream_t stream) {
   TcArgs a;
-  a.x = static_cast<const uint16_t*>(x);
   a.ldx = ldx;
   a.w = static_cast<const uint4*>(w);
   a.scale = static_cast<const uint32_t*>(scale);
   a.zero = static_cast<const uint8_t*>(zero);
   a.bias = bias;
-  a.out = static_cast<uint16_t*>(out);
   const uint64_t group_tiles = group == 32 ? 1 : static_cast<uint64_t>(group / 64);
   a.tiles_inv = static_cast<uint32_t>(((1ull << 31) + group_tiles - 1) / group_tiles);
-  a.M = static_cast<int>(M);
   a.N = static_cast<int>(N);
   a.K = static_cast<int>(K);
   a.groups = static_cast<int>(K / group);
   a.epilogue = epilogue;
   a.bias_dtype = bias_dtype;
-  const int64_t bx = (N + 127) / 128, by = plan.by;
+  const int64_t bx = (N + 127) / 128;
   a.tokens = plan.tokens;
   a.ks = plan.ks;
-  if (by > 65535) return HY3D_ERR_SHAPE;
   const bool plain = !zero, sub = group == 32;
   const int stage_bytes = 2 * a.tokens * 128, rings = kUnpackWarps * ring_depth(sub ? 2 : 1, plain) * slot_bytes(sub ? 2 : 1, plain);
   a.d_cols = (a.tokens + 31) / 32 * 32;
@@ -501,15 +497,10 @@ int gemm(const void* x, int x_dtype, int64_t ldx, const void* w, const void* sca
   smem += 1024;
   // One CTA per SM: each takes all 512 columns of tensor memory, so a second could only wait for them.
   if (smem < 120 * 1024) smem = 120 * 1024;
-  CUtensorMap tm_x;
-  int rc = encode_tmap_2d_u8(&tm_x, x, static_cast<uint64_t>(2 * K), static_cast<uint64_t>(M), static_cast<uint64_t>(2 * ldx), 128,
-                             static_cast<uint32_t>(a.tokens), 128);
-  if (rc != HY3D_OK) return rc;
   const TcFn kernel = x_dtype == HY3D_BF16 ? tc_kernel_of<true>(sub, plain) : tc_kernel_of<false>(sub, plain);
-  rc = ensure_max_smem(reinterpret_cast<const void*>(kernel), 226 * 1024);
+  int rc = ensure_max_smem(reinterpret_cast<const void*>(kernel), 226 * 1024);
   if (rc != HY3D_OK) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(bx * a.ks), static_cast<unsigned>(by));
   cfg.blockDim = dim3(kTcThreads);
   cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = stream;
@@ -520,9 +511,21 @@ int gemm(const void* x, int x_dtype, int64_t ldx, const void* w, const void* sca
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = a.ks > 1 ? 2 : 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, a, tm_x) != cudaSuccess) {
-    cudaGetLastError();
-    return HY3D_ERR_CUDA;
+  const int64_t n_out = epilogue == HY3D_EPI_GEGLU ? N / 2 : N, most = kMaxGridY * a.tokens;
+  for (int64_t first = 0; first < M; first += most) {      // as many rows as a grid has places in y
+    const int64_t rows = M - first < most ? M - first : most;
+    a.x = static_cast<const uint16_t*>(x) + first * ldx;
+    a.out = static_cast<uint16_t*>(out) + first * n_out;
+    a.M = static_cast<int>(rows);
+    CUtensorMap tm_x;
+    rc = encode_tmap_2d_u8(&tm_x, a.x, static_cast<uint64_t>(2 * K), static_cast<uint64_t>(rows), static_cast<uint64_t>(2 * ldx), 128,
+                           static_cast<uint32_t>(a.tokens), 128);
+    if (rc != HY3D_OK) return rc;
+    cfg.gridDim = dim3(static_cast<unsigned>(bx * a.ks), static_cast<unsigned>((rows + a.tokens - 1) / a.tokens));
+    if (cudaLaunchKernelEx(&cfg, kernel, a, tm_x) != cudaSuccess) {
+      cudaGetLastError();
+      return HY3D_ERR_CUDA;
+    }
   }
   return HY3D_OK;
 }

@@ -23,6 +23,7 @@ namespace {
 constexpr int kWarps = 16, kThreads = 32 * kWarps;
 constexpr int kMaxTrips = 8;
 constexpr int kSmem = 226 * 1024;
+constexpr int64_t kMaxGridY = 65535;
 constexpr int kTiles = 4, kStages = 2;      // tiles of a stage, stages of a warp's ring
 // Bytes of a stage for one block of rows: codes, scales, zero points.
 __host__ __device__ constexpr int stage_row(int sub, bool plain) { return kTiles * (512 + 32 * sub + (plain ? 0 : 16 * sub)); }
@@ -347,7 +348,7 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int64_t by, int r, int sub, bool p
 // The kernel of gemm_w4.cu, and how it would run a layer.
 struct TcPlan {
   int tokens, ks;
-  int64_t by, cycles;
+  int64_t cycles;
 };
 TcPlan tc_plan(int64_t M, int64_t N, int64_t K);
 int gemm(const void* x, int x_dtype, int64_t ldx, const void* w, const void* scale, const void* zero, int64_t group, const void* bias,
@@ -382,17 +383,13 @@ int linear(const void* x, int x_dtype, int64_t ldx, const void* w, const void* s
     if (M > 64 || tc.cycles < p.cycles)
       return gemm(x, x_dtype, ldx, w, scale, zero, group, bias, bias_dtype, out, M, N, K, epilogue, tc, stream);
   }
-  if (p.by > 65535) return HY3D_ERR_SHAPE;
   Args a;
-  a.x = static_cast<const uint16_t*>(x);
   a.ldx = ldx;
   a.w = static_cast<const uint4*>(w);
   a.scale = static_cast<const uint32_t*>(scale);
   a.zero = static_cast<const uint8_t*>(zero);
   a.bias = bias;
   a.bias_dtype = bias_dtype;
-  a.out = static_cast<uint16_t*>(out);
-  a.M = static_cast<int>(M);
   a.N = static_cast<int>(N);
   a.K = static_cast<int>(K);
   a.groups = static_cast<int>(K / group);
@@ -408,16 +405,24 @@ int linear(const void* x, int x_dtype, int64_t ldx, const void* w, const void* s
   rc = ensure_max_smem(reinterpret_cast<const void*>(kernel), 227 * 1024);
   if (rc != HY3D_OK) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.bx), static_cast<unsigned>(p.by));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = static_cast<size_t>(p.smem);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1] = {pdl_attribute()};
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) {
-    cudaGetLastError();
-    return HY3D_ERR_CUDA;
+  // A launch takes as many rows as a grid has places in y; the next goes on behind them.
+  const int64_t n_out = epilogue == HY3D_EPI_GEGLU ? N / 2 : N, most = kMaxGridY * p.tokens;
+  for (int64_t first = 0; first < M; first += most) {
+    const int64_t rows = M - first < most ? M - first : most;
+    a.x = static_cast<const uint16_t*>(x) + first * ldx;
+    a.out = static_cast<uint16_t*>(out) + first * n_out;
+    a.M = static_cast<int>(rows);
+    cfg.gridDim = dim3(static_cast<unsigned>(p.bx), static_cast<unsigned>((rows + p.tokens - 1) / p.tokens));
+    if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) {
+      cudaGetLastError();
+      return HY3D_ERR_CUDA;
+    }
   }
   return HY3D_OK;
 }

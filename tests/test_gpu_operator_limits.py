@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_operators import DEV, HALF, TINY, _gen, _within
+from test_gpu_operators import DEV, HALF, TINY, _check_int4, _gen, _int4, _within
 from test_operator_limits_host import _frequencies_of_many_digits, _pi
 
 pytestmark = pytest.mark.gpu
@@ -107,3 +107,25 @@ def test_rotary_far_positions_against_angles_of_many_digits(rotary, interleaved,
     join = (lambda a, b: torch.stack([a, b], -1).flatten(-2)) if interleaved else (lambda a, b: torch.cat([a, b], -1))
     ref, tol = join(y, z), join(tol, tol)
     _within(got, ref, tol + HALF[torch.float16] * (ref.abs() + tol) + TINY[torch.float16])
+
+
+@pytest.mark.parametrize("m,k,n,group,scales", [(8 * 65535 + 9, 64, 32, 32, torch.float16), (2 * 65535 + 1, 32768, 16, 1024, torch.float16),
+                                                (256 * 65535 + 300, 64, 16, 64, torch.bfloat16)])
+def test_int4_more_rows_than_a_grid_has_blocks(qu, m, k, n, group, scales):
+    """Scales of the activations' type and of the other: every row gets its answer, also behind the last block of a grid."""
+    g = _gen(k)
+    codes = torch.randint(0, 16, (n, k), generator=g, device=DEV)
+    scale = (torch.rand(n, k // group, generator=g, device=DEV) * 0.02 + 0.001).to(scales)
+    layer = qu.Int4Linear.from_codes(codes, scale)
+    w = layer.dequantize_weight().double()
+    x = torch.empty(m, k, device=DEV, dtype=torch.bfloat16)
+    some = torch.randn(4096, k, generator=g, device=DEV).bfloat16()
+    at = [0, m // 2 - 2048, m - 4096]
+    x.zero_()
+    for i in at:
+        x[i:i + 4096] = some
+    y = layer(x)
+    assert y.shape == (m, n)
+    for i in at:
+        _check_int4(layer, w, None, some, y[i:i + 4096])
+    assert not bool(y[4096:at[1]].any()) and not bool(y[at[1] + 4096:at[2]].any())
