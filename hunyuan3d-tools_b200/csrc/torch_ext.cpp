@@ -493,7 +493,7 @@ PyObject* quantize_weight(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // decline.
 struct Names {
   PyObject *w4, *zero, *dict, *buffers, *parameters, *mode, *epilogue, *bias, *wq, *scale, *comp, *meta, *forward, *compiled, *weight,
-      *eps, *fused, *silu, *groups, *shape, *dtype, *q, *act_scale, *conv_groups;
+      *eps, *fused, *silu, *groups, *shape, *dtype, *q, *act_scale, *conv_groups, *normalized_shape;
   PyObject* hooks[4];
 } names;
 struct Registered {
@@ -510,7 +510,7 @@ bool intern_names() {
       {&names.comp, "weight_sparse_comp"}, {&names.meta, "weight_sparse_meta"}, {&names.forward, "forward"},
       {&names.compiled, "_compiled_call_impl"}, {&names.weight, "weight"}, {&names.eps, "eps"}, {&names.fused, "fused"},
       {&names.silu, "silu"}, {&names.groups, "num_groups"}, {&names.shape, "shape"}, {&names.dtype, "dtype"},
-      {&names.q, "q"}, {&names.w4, "weight_int4"}, {&names.zero, "weight_zero"}, {&names.conv_groups, "groups"}, {&names.act_scale, "scale"}, {&names.hooks[0], "_backward_hooks"},
+      {&names.q, "q"}, {&names.normalized_shape, "normalized_shape"}, {&names.w4, "weight_int4"}, {&names.zero, "weight_zero"}, {&names.conv_groups, "groups"}, {&names.act_scale, "scale"}, {&names.hooks[0], "_backward_hooks"},
       {&names.hooks[1], "_backward_pre_hooks"}, {&names.hooks[2], "_forward_hooks"}, {&names.hooks[3], "_forward_pre_hooks"}};
   for (auto& n : all)
     if (!(*n.at = PyUnicode_InternFromString(n.text))) return false;
@@ -758,6 +758,11 @@ PyObject* rms_call(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int code = half_code(x->scalar_type());
   const int64_t K = x->size(-1), M = K > 0 ? x->numel() / K : 0;
   if (code < 0 || M <= 0 || (K & 7) || K > 16384) return none();
+  // the module's own width: a weight need not tell it
+  PyObject* widths = PyDict_GetItemWithError(dict, names.normalized_shape);
+  long width = 0;
+  if (!widths || !PyTuple_Check(widths) || PyTuple_GET_SIZE(widths) != 1 || !small_int(PyTuple_GET_ITEM(widths, 0), K, K, &width))
+    return none();
   const Affine f(gamma, Py_None, K, x->device());
   uintptr_t at16 = reinterpret_cast<uintptr_t>(x->const_data_ptr()) | reinterpret_cast<uintptr_t>(f.gamma);
   if (add) at16 |= reinterpret_cast<uintptr_t>(add->const_data_ptr());

@@ -5,6 +5,7 @@ import math
 
 import pytest
 import torch
+import torch.nn as nn
 
 from test_gpu_operators import DEV, HALF, TINY, _check_int4, _gen, _int4, _within
 from test_operator_limits_host import _frequencies_of_many_digits, _pi
@@ -129,3 +130,17 @@ def test_int4_more_rows_than_a_grid_has_blocks(qu, m, k, n, group, scales):
     for i in at:
         _check_int4(layer, w, None, some, y[i:i + 4096])
     assert not bool(y[4096:at[1]].any()) and not bool(y[at[1] + 4096:at[2]].any())
+
+
+def test_norm_of_another_width_is_refused_with_any_weight(qu):
+    """Also once the native path is loaded, where the weight does not tell the width (there is none, or it was replaced)."""
+    x, wide = torch.randn(4, 64, device=DEV).half(), torch.randn(4, 128, device=DEV).half()
+    for cls in (qu.AddRMSNorm, qu.Int8RMSNorm):
+        for norm in (cls(nn.RMSNorm(64, eps=1e-6, elementwise_affine=False)), cls(nn.RMSNorm(64, eps=1e-6, device=DEV))):
+            norm(x)                                     # loads the native path
+            for weight in (None, nn.Parameter(torch.ones(128, device=DEV), requires_grad=False)):
+                norm.weight = weight
+                with pytest.raises(RuntimeError, match="64 dimensions"):
+                    norm(wide)
+                with pytest.raises(RuntimeError, match="64 dimensions"):
+                    norm(wide, wide)
