@@ -747,8 +747,8 @@ PyObject* rms_call(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const bool codes = Py_TYPE(a[0]) == rmsnorm_classes[1].type;
   PyObject* dict = plain_module(a[0], rmsnorm_classes[codes]);
   PyObject* params = dict ? PyDict_GetItemWithError(dict, names.parameters) : nullptr;
-  PyObject* eps = dict ? PyDict_GetItemWithError(dict, names.eps) : nullptr;
-  if (!params || !PyDict_Check(params) || !eps || !PyFloat_Check(eps)) return none();
+  PyObject* peps = dict ? PyDict_GetItemWithError(dict, names.eps) : nullptr;
+  if (!params || !PyDict_Check(params) || !peps || (peps != Py_None && !PyFloat_Check(peps))) return none();
   PyObject* gamma = PyDict_GetItemWithError(params, names.weight);
   const at::Tensor *x = plain(a[1]), *add = a[2] == Py_None ? nullptr : plain(a[2]);
   if (!gamma || !x || x->dim() < 1 || wants_gradient(*x)) return none();
@@ -763,6 +763,8 @@ PyObject* rms_call(PyObject*, PyObject* const* a, Py_ssize_t n) {
   long width = 0;
   if (!widths || !PyTuple_Check(widths) || PyTuple_GET_SIZE(widths) != 1 || !small_int(PyTuple_GET_ITEM(widths, 0), K, K, &width))
     return none();
+  // None stands for the spacing of x's type at 1, as in nn.RMSNorm
+  const float eps = peps != Py_None ? static_cast<float>(PyFloat_AS_DOUBLE(peps)) : code == HY3D_BF16 ? 0x1p-7f : 0x1p-10f;
   const Affine f(gamma, Py_None, K, x->device());
   uintptr_t at16 = reinterpret_cast<uintptr_t>(x->const_data_ptr()) | reinterpret_cast<uintptr_t>(f.gamma);
   if (add) at16 |= reinterpret_cast<uintptr_t>(add->const_data_ptr());
@@ -778,7 +780,7 @@ PyObject* rms_call(PyObject*, PyObject* const* a, Py_ssize_t n) {
     y = at::Tensor(at::detail::empty_cuda(x->sizes(), x->scalar_type(), x->device(), std::nullopt));
   }
   const int rc = api.hy3d_rmsnorm(x->const_data_ptr(), K, add ? add->const_data_ptr() : nullptr, K, add ? sum.mutable_data_ptr() : nullptr,
-                                  code, M, K, f.gamma, f.code, static_cast<float>(PyFloat_AS_DOUBLE(eps)),
+                                  code, M, K, f.gamma, f.code, eps,
                                   codes ? nullptr : y.mutable_data_ptr(), codes ? q.mutable_data_ptr<int8_t>() : nullptr,
                                   codes ? s.mutable_data_ptr<float>() : nullptr, st);
   if (rc != HY3D_OK) return failed("hy3d_rmsnorm", rc);

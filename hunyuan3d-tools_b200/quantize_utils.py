@@ -226,7 +226,10 @@ class AddRMSNorm(nn.Module):
             raise RuntimeError(f"{type(self).__name__} normalises the last dimension only")
         self.normalized_shape = tuple(norm.normalized_shape)
         self.eps = norm.eps
-        self.weight = norm.weight
+        if norm.weight is None:
+            self.register_parameter("weight", None)
+        else:
+            self.weight = norm.weight
         self._ik = None
 
     def __call__(self, x, add=None):

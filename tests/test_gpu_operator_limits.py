@@ -7,7 +7,7 @@ import pytest
 import torch
 import torch.nn as nn
 
-from test_gpu_operators import DEV, HALF, TINY, _check_int4, _gen, _int4, _within
+from test_gpu_operators import DEV, HALF, TINY, _check_int4, _check_norm, _gen, _int4, _within
 from test_operator_limits_host import _frequencies_of_many_digits, _pi
 
 pytestmark = pytest.mark.gpu
@@ -144,3 +144,22 @@ def test_norm_of_another_width_is_refused_with_any_weight(qu):
                     norm(wide)
                 with pytest.raises(RuntimeError, match="64 dimensions"):
                     norm(wide, wide)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("affine", [False, True])
+def test_norms_with_the_default_eps_or_without_weight_take_the_direct_way(qu, ik, monkeypatch, dtype, affine):
+    x = torch.randn(6, 320, generator=_gen(5), device=DEV).to(dtype) * 2.0 ** -6      # small, so that eps counts
+    norm = nn.RMSNorm(320, elementwise_affine=affine).to(DEV, dtype)
+    half, codes = qu.AddRMSNorm(norm), qu.Int8RMSNorm(norm)
+    want, want_q = half.forward(x), codes.forward(x)      # the binding's answer
+    _check_norm(x, None, norm.weight, torch.finfo(dtype).eps, None, want)
+
+    def refuse(*a, **k):
+        raise AssertionError("the Python binding was called")
+    monkeypatch.setattr(type(ik), "rmsnorm", refuse)
+    assert torch.equal(half(x), want)
+    total, y = half(x, x)
+    assert torch.equal(total, x + x)
+    got = codes(x)
+    assert torch.equal(got.q, want_q.q) and torch.equal(got.scale, want_q.scale)
