@@ -281,6 +281,7 @@ class _Base:
         if gamma is not None:
             if gamma.numel() != K or gamma.device != x.device or gamma.dtype not in half + (torch.float32,):
                 raise RuntimeError(f"rmsnorm: weight must have {K} values of fp16, bf16 or fp32 on {x.device}")
+            self._no_tangent(gamma, "rmsnorm: weight")
             gamma = gamma.detach().contiguous()
             if gamma.data_ptr() % 16:
                 gamma = gamma.clone()
@@ -309,6 +310,12 @@ class _Base:
     def _no_gradient(t, what):
         if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{what} requires a gradient, and none is recorded here: call under torch.no_grad() or detach it")
+        _Base._no_tangent(t, what)
+
+    @staticmethod
+    def _no_tangent(t, what):
+        if torch._C._is_fwd_grad_enabled() and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what} carries a forward-mode gradient, and none is recorded here: unpack it first")
 
     def dequantize_rows(self, q, scale, dtype):
         """int8 codes (M,K) and scales (M) -> the (M,K) values they stand for, rounded to fp16 or bf16."""

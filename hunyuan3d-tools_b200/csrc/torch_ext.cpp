@@ -19,6 +19,7 @@
 #include <ATen/Context.h>
 #include <ATen/autocast_mode.h>
 #include <ATen/core/Tensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
@@ -673,8 +674,13 @@ PyObject* norm_call(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// A tensor whose gradient a caller expects, and none of these functions records.
-bool wants_gradient(const at::Tensor& t) { return t.requires_grad() && c10::GradMode::is_enabled(); }
+// A tensor whose gradient a caller expects, and none of these functions records: backwards, or along a forward-mode tangent.
+bool has_tangent(const at::Tensor& t) {
+  return t.unsafeGetTensorImpl()->autograd_meta() && c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined();
+}
+bool wants_gradient(const at::Tensor& t) {
+  return t.unsafeGetTensorImpl()->autograd_meta() && ((t.requires_grad() && c10::GradMode::is_enabled()) || has_tangent(t));
+}
 
 // The 4-bit layer of instance dictionary `dict` on a tensor.
 PyObject* int4_of(PyObject* layer, PyObject* dict, PyObject* px) {
@@ -732,7 +738,7 @@ PyObject* int4_call(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 // int4_forward(layer, x) -> y | None: Int4Linear.forward, also of subclasses
 PyObject* int4_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 2) return none();
+  if (n != 2 || torch::jit::tracer::isTracing()) return none();
   PyObject* dict = PyObject_GetAttr(a[0], names.dict);
   if (!dict) return nullptr;
   Py_DECREF(dict);
@@ -768,7 +774,7 @@ PyObject* rms_call(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Affine f(gamma, Py_None, K, x->device());
   uintptr_t at16 = reinterpret_cast<uintptr_t>(x->const_data_ptr()) | reinterpret_cast<uintptr_t>(f.gamma);
   if (add) at16 |= reinterpret_cast<uintptr_t>(add->const_data_ptr());
-  if (!f.ok || (at16 & 15)) return none();
+  if (!f.ok || (at16 & 15) || (gamma != Py_None && has_tangent(THPVariable_Unpack(gamma)))) return none();
   c10::cuda::CUDAGuard guard(x->device());
   cudaStream_t st = c10::cuda::getCurrentCUDAStream(x->device().index()).stream();
   at::Tensor sum, y, q, s;
@@ -884,7 +890,7 @@ bool apart(const Turned& a, const Turned& b, int64_t dim) {
 // (head dimensions, rotated ones, axes, interleaved, turns, axis of each pair, amplitude)
 PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t argc) {
   HANDLE_TH_ERRORS
-  if (argc != 7 || !PyTuple_CheckExact(a[0]) || PyTuple_GET_SIZE(a[0]) != 7) return none();
+  if (argc != 7 || !PyTuple_CheckExact(a[0]) || PyTuple_GET_SIZE(a[0]) != 7 || torch::jit::tracer::isTracing()) return none();
   PyObject* const* plan = &PyTuple_GET_ITEM(a[0], 0);
   long dim = 0, rot = 0, axes = 0;
   if (!small_int(plan[0], 1, 1 << 24, &dim) || !small_int(plan[1], 2, 512, &rot) || !small_int(plan[2], 1, 255, &axes) ||

@@ -211,6 +211,11 @@ class Int8LayerNorm(nn.Module):
         return f"{self.normalized_shape}, eps={self.eps}, output=int8 codes + per-token scales"
 
 
+def _not_traced(layer):
+    if torch.jit.is_tracing():
+        raise RuntimeError(f"{type(layer).__name__} cannot be traced: the trace would hold its output as a constant")
+
+
 class AddRMSNorm(nn.Module):
     """``nn.RMSNorm`` over the last dimension, optionally of ``x + add``, in one kernel: ``norm(x)`` returns the normalised
     activations, ``norm(x, add)`` returns ``(x + add, normalised)``, both in x's type -- a pre-norm block's residual stream
@@ -241,6 +246,7 @@ class AddRMSNorm(nn.Module):
         return super().__call__(x) if add is None else super().__call__(x, add)
 
     def forward(self, x: torch.Tensor, add: torch.Tensor | None = None):
+        _not_traced(self)
         if self._ik is None:
             _load_native()
             from .csrc.build import load_int8_kernels
@@ -818,6 +824,7 @@ class Int4Linear(nn.Module):
         y = (_NATIVE or _load_native()).int4_forward(self, x)
         if y is not None:
             return y
+        _not_traced(self)
         if isinstance(x, QuantizedActivation):
             raise RuntimeError("Int4Linear takes 16-bit activations, not int8 codes")
         if not x.is_cuda:

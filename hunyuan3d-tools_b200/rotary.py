@@ -113,6 +113,8 @@ class RotaryPositions:
 
     def _refuse(self, q, k, positions, offset, inplace):
         """Raises with what is wrong with a call that the native path declined."""
+        if torch.jit.is_tracing():
+            raise RuntimeError("rotary: the call cannot be traced: the trace would hold its output as a constant")
         tensors = [("q", q)] + ([("k", k)] if k is not None else [])
         for name, t in tensors:
             if not isinstance(t, torch.Tensor) or not t.is_cuda:
@@ -129,6 +131,8 @@ class RotaryPositions:
             if t.requires_grad and torch.is_grad_enabled():
                 raise RuntimeError(f"rotary: {name} requires a gradient, and none is recorded here: call under "
                                    "torch.no_grad() or detach it")
+            if torch._C._is_fwd_grad_enabled() and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"rotary: {name} carries a forward-mode gradient, and none is recorded here: unpack it first")
         if positions is not None:
             shape, lead, n = tuple(getattr(positions, "shape", ())), tuple(q.shape[:-2]), q.shape[-3]
             ends = ((),) if len(self.axes) == 1 else ()

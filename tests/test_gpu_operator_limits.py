@@ -5,6 +5,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 import torch.nn as nn
 
 from test_gpu_operators import DEV, HALF, TINY, _check_int4, _check_norm, _gen, _int4, _within
@@ -163,3 +164,28 @@ def test_norms_with_the_default_eps_or_without_weight_take_the_direct_way(qu, ik
     assert torch.equal(total, x + x)
     got = codes(x)
     assert torch.equal(got.q, want_q.q) and torch.equal(got.scale, want_q.scale)
+
+
+def test_tangents_and_traced_calls_are_refused(qu, rotary):
+    """A forward-mode tangent would be dropped, and a trace would hold the answer as a constant."""
+    layer, _, _ = _int4(qu, 64, 128, 64, False, True, torch.float16, 7)
+    norm = nn.RMSNorm(128, eps=1e-6, device=DEV, dtype=torch.float16).requires_grad_(False)
+    half, codes, r = qu.AddRMSNorm(norm), qu.Int8RMSNorm(norm), rotary.RotaryPositions(64)
+    x, q = torch.randn(4, 128, device=DEV).half(), torch.randn(4, 2, 64, device=DEV).half()
+    calls = [(layer, (x,)), (half, (x,)), (half, (x, x)), (codes, (x,)), (r, (q,)), (r, (q, q))]
+    for f, args in calls:
+        f(*args)
+    with fwAD.dual_level():
+        for f, args in calls:
+            for i in range(len(args)):
+                dual = [fwAD.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate(args)]
+                with pytest.raises(RuntimeError, match="gradient"):
+                    f(*dual)
+                with torch.no_grad(), pytest.raises(RuntimeError, match="gradient"):      # no_grad leaves tangents on
+                    f(*dual)
+            f(*args)
+    outer = lambda f: (lambda *a: f(*a).q if f is codes else f(*a))
+    for f, args in calls:
+        with pytest.raises(RuntimeError, match="trace"):
+            torch.jit.trace(outer(f), args, check_trace=False)
+        f(*args)
