@@ -291,6 +291,8 @@ int rmsnorm(const void* x, int64_t ldx, const void* add, int64_t ld_add, void* s
   const uintptr_t at16 = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(add) | reinterpret_cast<uintptr_t>(add ? sum : nullptr) |
                          reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(gamma);
   if ((at16 & 15) || (reinterpret_cast<uintptr_t>(q) & 7)) return HY3D_ERR_SHAPE;
+  const int rc = device_ok();
+  if (rc != HY3D_OK) return rc;
   Args a;
   a.x = static_cast<const uint16_t*>(x);
   a.add = static_cast<const uint16_t*>(add);

@@ -88,3 +88,16 @@ def test_rotary_fractions_are_the_nearest(rotary, d, base, scaling):
         for t, e, w in zip(memoryview(r._turns).cast("Q"), exact, r.frequencies, strict=True):
             assert abs(t - e) <= decimal.Decimal("0.500001")
             assert w == float(e / 2 ** 64 * (2 * _pi()))
+
+
+# ---- the device is asked for ------------------------------------------------------------------
+@pytest.mark.parametrize("name,entries", [("rmsnorm.cu", ("rmsnorm", "dequantize_rows")), ("rotary.cu", ("apply",)), ("linear_w4.cu", ("linear",))])
+def test_entry_points_ask_for_the_device_before_they_launch(build_mod, name, entries):
+    """So that another GPU is answered with its own status, not with that of a launch that failed.  Read from the sources,
+    as no other GPU is at hand."""
+    with open(os.path.join(os.path.dirname(build_mod.__file__), name)) as f:
+        functions = re.split(r"^}", f.read(), flags=re.M)
+    for entry in entries:
+        body, = [b for b in functions if re.search(rf"^int {entry}\(", b, flags=re.M)]
+        body = body[re.search(rf"^int {entry}\(", body, flags=re.M).start():]
+        assert re.search(r"= device_ok\(\);\s+if \(rc != HY3D_OK\) return rc;", body), f"{name}: {entry}"
