@@ -623,6 +623,16 @@ def _unpack_groups(v: torch.Tensor) -> torch.Tensor:
     return v.view(blocks, groups, 8, 2).permute(0, 3, 2, 1).reshape(blocks * 16, groups)
 
 
+def _int4_limits(scale, zero=None):
+    """What the kernels rely on and these values do not keep, or None: every ``scale * (code - zero)`` is a number of the
+    scale's type, and a zero point has four bits."""
+    if scale.numel() and not scale.is_meta and not bool((scale.detach().float().abs() <= torch.finfo(scale.dtype).max / 16).all()):
+        return f"a scale is not finite or above a sixteenth of the largest {scale.dtype}"
+    if zero is not None and zero.numel() and not zero.is_meta and (int(zero.min()) < 0 or int(zero.max()) > 15):
+        return "a zero point does not lie between 0 and 15"
+    return None
+
+
 class Int4Linear(nn.Module):
     """``nn.Linear`` with 4-bit weights and group scales, for layers that see few rows at a time: the weights are read at a
     quarter of their 16-bit size, the activations stay in 16 bits::
@@ -674,12 +684,11 @@ class Int4Linear(nn.Module):
                                f"got {tuple(codes.shape)} of {codes.dtype} and {tuple(scale.shape)}")
         if zero is not None and (zero.shape != scale.shape or zero.is_floating_point()):
             raise RuntimeError("Int4Linear.from_codes takes whole zero points in the shape of the scales")
-        for name, t in (("codes", codes), ("zero", zero)):
-            if t is not None and t.numel() and (int(t.min()) < 0 or int(t.max()) > 15):
-                raise RuntimeError(f"Int4Linear.from_codes: {name} must lie between 0 and 15")
-        if scale.numel() and scale.is_floating_point() \
-                and not bool((scale.detach().float().abs() <= torch.finfo(scale.dtype).max / 16).all()):
-            raise RuntimeError("Int4Linear.from_codes: a scale is not finite or above a sixteenth of its type's largest number")
+        if codes.numel() and (int(codes.min()) < 0 or int(codes.max()) > 15):
+            raise RuntimeError("Int4Linear.from_codes: codes must lie between 0 and 15")
+        wrong = _int4_limits(scale, zero) if scale.is_floating_point() else None
+        if wrong is not None:
+            raise RuntimeError(f"Int4Linear.from_codes: {wrong}")
         n, k = codes.shape
         if bias is not None and tuple(bias.shape) != (n,):
             raise RuntimeError(f"Int4Linear.from_codes: bias must have {n} entries, got {tuple(bias.shape)}")
@@ -800,16 +809,51 @@ class Int4Linear(nn.Module):
         self.epilogue = state.get("epilogue", "linear")
 
     def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
-        # Group size, zero points, bias and type are the checkpoint's.
-        src = state_dict.get(prefix + "weight_int4")
+        # Group size, zero points, bias and type are the checkpoint's (not a wider type, which the kernels do not take).
+        # Values that the kernels do not take either are refused, and the layer stays as it was.
+        half = (torch.float16, torch.bfloat16)
+        src, scale, zero = (state_dict.get(prefix + name) for name in ("weight_int4", "weight_scale", "weight_zero"))
+        if scale is not None or zero is not None:
+            kept = scale is not None and (local_metadata.get("assign_to_params_buffers", False) or scale.dtype in half)
+            scale = self.weight_scale if scale is None else scale if kept else scale.to(self.weight_scale.dtype)
+            wrong = self._bad_groups(scale, zero)
+            if wrong is not None:
+                error_msgs.append(f"{prefix}weight_scale: {wrong}")
+                return
         if src is not None and tuple(src.shape) == tuple(self.weight_int4.shape):
             for name in ("weight_scale", "weight_zero", "bias"):
                 src, cur = state_dict.get(prefix + name), getattr(self, name)
                 if src is None:
                     self.register_buffer(name, None if name != "weight_scale" else cur)
                 elif cur is None or cur.shape != src.shape or cur.dtype != src.dtype:
-                    self.register_buffer(name, torch.empty(src.shape, dtype=src.dtype, device=self.weight_int4.device))
+                    dtype = self.weight_scale.dtype if name == "weight_scale" and src.dtype not in half else src.dtype
+                    self.register_buffer(name, torch.empty(src.shape, dtype=dtype, device=self.weight_int4.device))
         super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+
+    def _bad_groups(self, scale, zero):
+        """What is wrong with these scales and zero points for this layer's weights, or None."""
+        shape = tuple(scale.shape)
+        if len(shape) != 3 or shape[::2] != (self.out_features // 16, 16) or shape[1] < 1 or self.in_features % shape[1]:
+            return f"scales of shape {shape} do not fit {self.in_features} inputs and {self.out_features} outputs"
+        group = self.in_features // shape[1]
+        if group < 32 or (group != 32 and group % 64):
+            return f"groups of {group} columns, expected 32 or a multiple of 64"
+        if not scale.is_floating_point():
+            return f"scales of {scale.dtype}, expected fp16 or bf16"
+        if zero is not None and (zero.shape != scale.shape or zero.dtype != torch.uint8):
+            return f"zero points of shape {tuple(zero.shape)} and {zero.dtype}, expected {shape} and uint8"
+        return _int4_limits(scale, zero)
+
+    def _apply(self, fn, recurse=True):
+        # ``half()`` and the like round the scales to another type, which may not hold them.
+        scale = self.weight_scale
+        super()._apply(fn, recurse)
+        if self.weight_scale.dtype != scale.dtype:
+            wrong = _int4_limits(self.weight_scale)
+            if wrong is not None:
+                self.weight_scale = scale
+                raise RuntimeError(f"Int4Linear: scales of {scale.dtype} cannot be converted: {wrong}")
+        return self
 
     # -- forward ------------------------------------------------------------------------
     def __call__(self, *args, **kwargs):

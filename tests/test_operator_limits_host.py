@@ -101,3 +101,61 @@ def test_entry_points_ask_for_the_device_before_they_launch(build_mod, name, ent
         body, = [b for b in functions if re.search(rf"^int {entry}\(", b, flags=re.M)]
         body = body[re.search(rf"^int {entry}\(", body, flags=re.M).start():]
         assert re.search(r"= device_ok\(\);\s+if \(rc != HY3D_OK\) return rc;", body), f"{name}: {entry}"
+
+
+# ---- what checkpoints and conversions bring ---------------------------------------------------
+def _int4_state(qu, dtype=torch.float16, zeros=True):
+    torch.manual_seed(4)
+    codes = torch.randint(0, 16, (32, 128))
+    zero = torch.randint(0, 16, (32, 2)) if zeros else None
+    layer = qu.Int4Linear.from_codes(codes, (torch.rand(32, 2) + 0.5).to(dtype), zero, torch.zeros(32))
+    return layer, {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in layer.state_dict().items()}
+
+
+@pytest.mark.parametrize("assign", [False, True])
+@pytest.mark.parametrize("name,value,match", [("weight_scale", 4096.0, "sixteenth"), ("weight_scale", float("inf"), "sixteenth"),
+                                              ("weight_scale", float("nan"), "sixteenth"), ("weight_zero", 16, "zero point"),
+                                              ("weight_zero", 255, "zero point")])
+def test_int4_checkpoints_outside_the_kernels_limits_are_refused(qu, assign, name, value, match):
+    layer, state = _int4_state(qu)
+    fresh = qu.Int4Linear(128, 32, group_size=64, symmetric=False)
+    before = {k: v.clone() for k, v in fresh.state_dict().items() if isinstance(v, torch.Tensor)}
+    state[name].view(-1)[7] = value
+    with pytest.raises(RuntimeError, match=match):
+        fresh.load_state_dict(state, assign=assign)
+    assert all(torch.equal(fresh.state_dict()[k], v) for k, v in before.items())
+    fresh.load_state_dict(layer.state_dict(), assign=assign)
+    assert torch.equal(fresh.dequantize_weight(), layer.dequantize_weight())
+
+
+def test_int4_checkpoints_of_other_shapes_and_types(qu):
+    layer, state = _int4_state(qu)
+    for bad in (dict(weight_scale=state["weight_scale"][:1]), dict(weight_scale=torch.ones(2, 3, 16).half()),
+                dict(weight_scale=torch.ones(2, 8, 16).half(), weight_zero=torch.zeros(2, 8, 16, dtype=torch.uint8)),
+                dict(weight_zero=state["weight_zero"][:, :1]), dict(weight_zero=state["weight_zero"].int())):
+        with pytest.raises(RuntimeError, match="weight_scale"):
+            qu.Int4Linear(128, 32).load_state_dict({**state, **bad})
+    wide = qu.Int4Linear(128, 32)            # scales that were kept in fp32 come back in the layer's type, which the kernels take
+    wide.load_state_dict({**state, "weight_scale": state["weight_scale"].float()})
+    assert wide.weight_scale.dtype == torch.float16 and torch.equal(wide.dequantize_weight(), layer.dequantize_weight())
+    wide.float().load_state_dict({**state, "weight_scale": state["weight_scale"].float()})      # and into a layer in fp32, as it is
+    assert wide.weight_scale.dtype == torch.float32 and torch.equal(wide.half().dequantize_weight(), layer.dequantize_weight())
+    with pytest.raises(RuntimeError, match="fp16 or bf16"):
+        qu.Int4Linear(128, 32).load_state_dict({**state, "weight_scale": torch.ones(2, 2, 16, dtype=torch.int32)}, assign=True)
+    with pytest.raises(RuntimeError, match="zero point"):
+        layer.load_state_dict({"weight_zero": torch.full((2, 2, 16), 16, dtype=torch.uint8)}, strict=False)
+
+
+def test_int4_conversions_that_lose_scales_are_refused(qu):
+    layer, _ = _int4_state(qu, torch.bfloat16)
+    layer.weight_scale[1, 0, 3] = 4096.0
+    kept = layer.weight_scale.clone()
+    for convert in (lambda m: m.half(), lambda m: m.to(torch.float16), lambda m: nn.Sequential(m).half()):
+        with pytest.raises(RuntimeError, match="sixteenth"):
+            convert(layer)
+        assert layer.weight_scale.dtype == torch.bfloat16 and torch.equal(layer.weight_scale, kept)
+    layer.weight_scale[1, 0, 3] = 4080.0
+    want = layer.dequantize_weight()
+    layer.float().half()
+    assert layer.weight_scale.dtype == torch.float16 and torch.equal(layer.dequantize_weight(), want)
+    layer.to("meta").half()
