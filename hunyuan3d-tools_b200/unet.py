@@ -206,6 +206,20 @@ class Attention(nn.Module):
     rotary = None
     rotary_positions = None
 
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        if self.rotary_positions is not None:       # to the module's device, in their own type
+            moved = {n: (t, fn(t)) for n, t in self.rotary_positions.items()}
+            self.rotary_positions = {n: v if v.dtype == t.dtype else t.to(v.device) for n, (t, v) in moved.items()}
+        return self
+
+    def _positions_of(self, n):
+        if self.rotary_positions is None:
+            return None
+        if n not in self.rotary_positions:
+            raise RuntimeError(f"no rotary positions for {n} tokens, only for {sorted(self.rotary_positions)}")
+        return self.rotary_positions[n]
+
     def forward(self, x, context=None, kv=None):
         """``kv``: keys and values of the context side by side, where the caller has them already."""
         b, n, c = x.shape
@@ -228,8 +242,7 @@ class Attention(nn.Module):
         q = q.view(b, n, self.heads, c // self.heads)
         k = k.view(b, m, self.heads, c // self.heads)
         if self.rotary is not None:       # into new tensors: a hook may have kept the projections' outputs
-            at = None if self.rotary_positions is None else self.rotary_positions[n]
-            q, k = self.rotary(q, k, at)
+            q, k = self.rotary(q, k, self._positions_of(n))
         q, k = q.transpose(1, 2), k.transpose(1, 2)
         v = v.view(b, m, self.heads, c // self.heads).transpose(1, 2)
         o = F.scaled_dot_product_attention(q, k, v)
@@ -489,13 +502,14 @@ def fuse_geglu_layers(model: nn.Module) -> int:
 
 def use_multiview_rotary(model: nn.Module, positions: dict, base: float = 10000.0, interleaved: bool = True, scaling=None) -> int:
     """Gives every multiview attention rotary positions: ``positions`` maps a number of tokens (views x height x width of a
-    level) to an int tensor (tokens) or (tokens, axes), such as (view, row, column) or a voxel's coordinates.  The head's
-    dimensions are shared out evenly among the axes.  Returns the number of attentions changed."""
+    level) to an int tensor (tokens) or (tokens, axes), such as (view, row, column) or a voxel's coordinates, which moves
+    with the model.  The head's dimensions are shared out evenly among the axes.  Returns the number of attentions changed."""
     from .rotary import RotaryPositions
     ends = {t.shape[1] if t.dim() == 2 else 1 for t in positions.values()}
-    if len(ends) != 1 or any(t.shape[0] != n for n, t in positions.items()):
-        raise RuntimeError("positions must map each number of tokens to that many positions, all of the same axes")
-    axes, count = ends.pop(), 0
+    if len(ends) != 1 or any(t.dim() not in (1, 2) or t.shape[0] != n or t.dtype not in (torch.int32, torch.int64)
+                             for n, t in positions.items()):
+        raise RuntimeError("positions must map each number of tokens to that many positions of int32 or int64, all of the same axes")
+    axes, plans = ends.pop(), []
     for blk in model.modules():
         if not isinstance(blk, TransformerBlock) or blk.num_views < 2:
             continue
@@ -503,10 +517,10 @@ def use_multiview_rotary(model: nn.Module, positions: dict, base: float = 10000.
         dim = blk.norm_mv.normalized_shape[0] // attn.heads
         pairs = dim // 2
         parts = [2 * (pairs // axes + (1 if i < pairs % axes else 0)) for i in range(axes)]
-        attn.rotary = RotaryPositions(dim, sum(parts), base, interleaved, parts, scaling)
-        attn.rotary_positions = dict(positions)
-        count += 1
-    return count
+        plans.append((attn, RotaryPositions(dim, sum(parts), base, interleaved, parts, scaling)))
+    for attn, plan in plans:
+        attn.rotary, attn.rotary_positions = plan, dict(positions)
+    return len(plans)
 
 
 def fuse_layernorm_quant(model: nn.Module) -> int:

@@ -159,3 +159,30 @@ def test_int4_conversions_that_lose_scales_are_refused(qu):
     layer.float().half()
     assert layer.weight_scale.dtype == torch.float16 and torch.equal(layer.dequantize_weight(), want)
     layer.to("meta").half()
+
+
+# ---- multiview positions -----------------------------------------------------------------------
+def test_multiview_positions_go_where_the_model_goes(pkg):
+    un = importlib.import_module(PKG + ".unet")
+    blk = un.TransformerBlock(128, 2, 128, 2)
+    given = {8: 500001 + torch.arange(8), 4: torch.arange(4).int()}
+    un.use_multiview_rotary(blk, given)
+    blk.to(torch.bfloat16).double().type(torch.float16)      # types of weights are not types of positions
+    assert [t.dtype for t in blk.attn_mv.rotary_positions.values()] == [torch.int64, torch.int32]
+    assert torch.equal(blk.attn_mv.rotary_positions[8], given[8])
+    nn.Sequential(blk).to("meta")
+    assert all(t.device.type == "meta" for t in blk.attn_mv.rotary_positions.values())
+    assert given[8].device.type == "cpu" and blk.attn1.rotary_positions is None
+
+
+def test_multiview_positions_that_are_missing_or_do_not_fit(pkg):
+    un = importlib.import_module(PKG + ".unet")
+    blk = un.TransformerBlock(128, 2, 128, 2)
+    un.use_multiview_rotary(blk, {8: torch.arange(8)})
+    with pytest.raises(RuntimeError, match="12 tokens.*8"):
+        blk.attn_mv(torch.zeros(1, 12, 128))
+    other = nn.Sequential(un.TransformerBlock(128, 2, 128, 2), un.TransformerBlock(128, 32, 128, 2))      # heads of 64, and of 4
+    for bad in ({8: torch.zeros(8, 3, dtype=torch.int64)}, {8: torch.zeros(8)}, {8: torch.zeros(8, 2, 2, dtype=torch.int64)}, {}):
+        with pytest.raises(RuntimeError):
+            un.use_multiview_rotary(other, bad)
+        assert all(b.attn_mv.rotary is None and b.attn_mv.rotary_positions is None for b in other)
