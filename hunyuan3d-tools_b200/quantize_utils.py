@@ -643,6 +643,8 @@ class Int4Linear(nn.Module):
     ``Int8Linear`` (same epilogues, ``concat``, ``interleave_geglu_rows``, checkpoints); the reference has no counterpart.
     Any number of rows; in_features % 64 == 0 and at most 32768, out_features % 16 == 0, groups of 32 or of a multiple of 64 columns that
     divides in_features.  CUDA fp16 / bf16 only; no gradient is recorded.
+    Scales of the activations' type are the fast case: with those of the other 16-bit type, right too, the weights are read and
+    unpacked again for every 8 rows.
 
     Buffers: ``weight_int4`` (N/16, K/64, 512) uint8, ``weight_scale`` (N/16, groups, 16), ``weight_zero`` likewise uint8 or
     None, in the kernel's order; ``codes()``, ``scales()`` and ``zeros()`` give them row by row."""
@@ -704,12 +706,13 @@ class Int4Linear(nn.Module):
 
     @staticmethod
     @torch.no_grad()
-    def from_linear(linear: nn.Linear, group_size: int = 64, symmetric: bool = True) -> "Int4Linear":
+    def from_linear(linear: nn.Linear, group_size: int = 64, symmetric: bool = True, dtype: torch.dtype | None = None) -> "Int4Linear":
         """Round-to-nearest quantisation of an ``nn.Linear``, group by group, with the scale as it is stored:
         symmetric ``scale = max|w| / 7``, codes ``round(w / scale) + 8``; otherwise ``scale = (max - min) / 15``, the range
-        widened to hold 0, and a zero point ``round(-min / scale)``."""
+        widened to hold 0, and a zero point ``round(-min / scale)``.  ``dtype``: type of the scales and the bias, that of the
+        activations to come (the layer's own by default, fp16 for an fp32 layer)."""
         n, k = linear.weight.shape
-        dt = _param_dtype(linear)
+        dt = _param_dtype(linear) if dtype is None else dtype
         with torch.device("meta"):
             Int4Linear(k, n, bias=False, dtype=dt, group_size=group_size)
         w = linear.weight.detach().float().view(n, k // group_size, group_size)
@@ -1009,10 +1012,11 @@ def quantize_model_mixed(model, min_features=128, sparse_min_k=None, verbose=Tru
     return stats
 
 
-def quantize_model_int4(model, min_features=128, group_size=64, symmetric=True, choose=None, verbose=True):
+def quantize_model_int4(model, min_features=128, group_size=64, symmetric=True, choose=None, verbose=True, dtype=None):
     """Replace ``nn.Linear`` layers with ``Int4Linear`` in place: those of at least ``min_features`` inputs and outputs that
     the layer's shape rules admit and, with ``choose``, those for which ``choose(name, layer)`` is true -- the ones that see
-    few rows (in the texture UNet ``lambda name, _: "time_emb" in name``); the other converters then take the rest."""
+    few rows (in the texture UNet ``lambda name, _: "time_emb" in name``); the other converters then take the rest.
+    ``dtype``: as for ``Int4Linear.from_linear``."""
     stats = {"total_params": 0, "quantized_params": 0, "skipped_params": 0, "num_replaced": 0, "kept_fp16": 0}
     for name, child in list(model.named_modules()):
         if not isinstance(child, nn.Linear) or not name:
@@ -1026,7 +1030,7 @@ def quantize_model_int4(model, min_features=128, group_size=64, symmetric=True, 
             stats["kept_fp16"] += 1
         else:
             parent = model.get_submodule(name.rpartition(".")[0])
-            setattr(parent, name.rpartition(".")[2], Int4Linear.from_linear(child, group_size, symmetric))
+            setattr(parent, name.rpartition(".")[2], Int4Linear.from_linear(child, group_size, symmetric, dtype))
             stats["quantized_params"] += num_params
             stats["num_replaced"] += 1
     if verbose:

@@ -202,7 +202,7 @@ int hy3d_rotary(const hy3d_rotary_side* sides, int n_sides, int dtype, int64_t b
  * those of words 2 and 3 32 more; nibble j < 4 of a word is its column 2j, nibble 4 + j its column 2j + 1.
  * scale: f16 / bf16 [N/16][K/group][16], place 2g for row g and 2g + 1 for row g + 8; finite, and scale * 15 within the range
  * of its type.  zero: the same places, a byte 0..15 each, or NULL for 8 throughout.  group: 32, or a multiple of 64; divides
- * K.  bias (N) or NULL.
+ * K.  bias (N) or NULL.  With scale of the other 16-bit type than x, the weights are read again for every 8 rows.
  * Epilogues as for the int8 GEMMs (HY3D_EPI_GEGLU: rows interleaved in blocks of 16, N / 2 columns out), GELU in its exact
  * form.  out: (M, N or N / 2) of x's type.  Requires K % 64 == 0, K <= 32768, N % 16 == 0 (% 32 GEGLU), 16-byte aligned x
  * rows, w, scale and zero, 8-byte aligned out.  No workspace.  No counterpart in the reference.

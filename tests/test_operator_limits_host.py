@@ -186,3 +186,22 @@ def test_multiview_positions_that_are_missing_or_do_not_fit(pkg):
         with pytest.raises(RuntimeError):
             un.use_multiview_rotary(other, bad)
         assert all(b.attn_mv.rotary is None and b.attn_mv.rotary_positions is None for b in other)
+
+
+# ---- the scales' type ----------------------------------------------------------------------------
+def test_int4_scales_take_the_type_that_is_asked_for(qu):
+    torch.manual_seed(5)
+    lin = nn.Linear(128, 128)
+    for dt in (torch.float16, torch.bfloat16):
+        for symmetric in (True, False):
+            layer = qu.Int4Linear.from_linear(lin, 64, symmetric, dtype=dt)
+            assert layer.weight_scale.dtype == dt and layer.bias.dtype == dt
+            # half a step for the code, or where the range ends for the zero point; there the scale's rounding 15 times too
+            step = layer.scales().float().repeat_interleave(64, 1)
+            assert bool(((layer.dequantize_weight() - lin.weight).abs() <= step * (0.5 + 15 * torch.finfo(dt).eps)).all())
+        net = nn.Sequential(nn.Linear(128, 128))
+        qu.quantize_model_int4(net, verbose=False, dtype=dt)
+        assert net[0].weight_scale.dtype == dt
+    assert qu.Int4Linear.from_linear(lin).weight_scale.dtype == torch.float16
+    with pytest.raises(RuntimeError, match="fp16 or bf16"):
+        qu.Int4Linear.from_linear(lin, dtype=torch.float32)
