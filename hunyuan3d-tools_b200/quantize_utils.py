@@ -55,6 +55,16 @@ def _kernel_unavailable(name, err):
 # ---------------------------------------------------------------------------------------
 _TC_MODULE = None
 _SP_MODULE = None
+_IK_MODULE = None
+
+
+def _load_ik():
+    """Lazy-load the quantise / normalise kernels.  Not kept by the modules, which can be copied and saved whole."""
+    global _IK_MODULE
+    if _IK_MODULE is None:
+        from .csrc.build import load_int8_kernels
+        _IK_MODULE = load_int8_kernels()
+    return _IK_MODULE
 
 
 def _load_tc():
@@ -161,8 +171,7 @@ class QuantizedActivation:
         """The values that the codes stand for, rounded to the activation's type."""
         y = (_NATIVE or _load_native()).dequantize(self.q, self.scale, self.dtype, self.shape)
         if y is None:
-            from .csrc.build import load_int8_kernels
-            y = load_int8_kernels().dequantize_rows(self.q, self.scale, self.dtype).reshape(self.shape)
+            y = _load_ik().dequantize_rows(self.q, self.scale, self.dtype).reshape(self.shape)
         return y
 
 
@@ -181,7 +190,6 @@ class Int8LayerNorm(nn.Module):
         self.eps = norm.eps
         self.weight = norm.weight
         self.bias = norm.bias
-        self._ik = None
 
     def __call__(self, *args, **kwargs):
         # The direct way to the kernel where no hook, subclass or tracer stands in it (1.5 us less host time).
@@ -198,13 +206,10 @@ class Int8LayerNorm(nn.Module):
             return QuantizedActivation(got[0], got[1], x.shape, x.dtype)
         if not x.is_cuda:
             raise RuntimeError("Int8LayerNorm runs on CUDA tensors only (no CPU fallback)")
-        if self._ik is None:
-            from .csrc.build import load_int8_kernels
-            self._ik = load_int8_kernels()
         x2 = x.reshape(-1, x.shape[-1])
         if not x2.is_contiguous():
             x2 = x2.contiguous()
-        q, s = self._ik.layernorm_quantize(x2, self.weight, self.bias, self.eps)
+        q, s = _load_ik().layernorm_quantize(x2, self.weight, self.bias, self.eps)
         return QuantizedActivation(q, s, x.shape, x.dtype)
 
     def extra_repr(self) -> str:
@@ -235,7 +240,6 @@ class AddRMSNorm(nn.Module):
             self.register_parameter("weight", None)
         else:
             self.weight = norm.weight
-        self._ik = None
 
     def __call__(self, x, add=None):
         # The direct way to the kernel where no hook, subclass or tracer stands in it.
@@ -247,16 +251,14 @@ class AddRMSNorm(nn.Module):
 
     def forward(self, x: torch.Tensor, add: torch.Tensor | None = None):
         _not_traced(self)
-        if self._ik is None:
+        if _NATIVE is None:
             _load_native()
-            from .csrc.build import load_int8_kernels
-            self._ik = load_int8_kernels()
         if isinstance(x, torch.Tensor) and tuple(x.shape[-1:]) != self.normalized_shape:
             raise RuntimeError(f"{type(self).__name__} normalises {self.normalized_shape[0]} dimensions, got {tuple(x.shape)}")
         eps = self.eps
         if eps is None:         # nn.RMSNorm's default
             eps = torch.finfo(x.dtype).eps if isinstance(x, torch.Tensor) and x.is_floating_point() else 0.0
-        total, y, q, s = self._ik.rmsnorm(x, self.weight, eps, add, codes=self._codes, normalised=not self._codes)
+        total, y, q, s = _load_ik().rmsnorm(x, self.weight, eps, add, codes=self._codes, normalised=not self._codes)
         if self._codes:
             y = QuantizedActivation(q, s, x.shape, x.dtype)
         return y if add is None else (total, y)

@@ -105,7 +105,6 @@ class GroupNormNHWC(nn.GroupNorm):
         super().__init__(num_groups, num_channels, eps=eps)
         self.silu = silu
         self.fused = False
-        self._ik = None
 
     def __call__(self, x, add=None):
         # The direct way to the kernel where no hook, subclass or tracer stands in it.
@@ -127,11 +126,8 @@ class GroupNormNHWC(nn.GroupNorm):
                 x, self.num_groups, p["weight"], p["bias"], self.eps, self.silu, add)
             if y is not None:
                 return y
-            if self._ik is None:
-                from .csrc.build import load_int8_kernels
-                self._ik = load_int8_kernels()
-            return self._ik.groupnorm_nhwc(x, self.num_groups, self.weight, self.bias, self.eps,
-                                           silu=self.silu, add=add)
+            return _qu._load_ik().groupnorm_nhwc(x, self.num_groups, self.weight, self.bias, self.eps,
+                                                 silu=self.silu, add=add)
         if add is not None:
             x = x + add[:, :, None, None]
         y = super().forward(x)

@@ -1,4 +1,5 @@
 """CPU: rules that the 4-bit layers, the RMSNorms and the rotary positions keep at their limits."""
+import contextlib
 import ctypes
 import decimal
 import importlib
@@ -205,3 +206,19 @@ def test_int4_scales_take_the_type_that_is_asked_for(qu):
     assert qu.Int4Linear.from_linear(lin).weight_scale.dtype == torch.float16
     with pytest.raises(RuntimeError, match="fp16 or bf16"):
         qu.Int4Linear.from_linear(lin, dtype=torch.float32)
+
+
+# ---- modules that have run can be copied --------------------------------------------------------
+def test_modules_keep_no_library_handle(qu, pkg, build_mod):
+    """A model is copied and saved whole also after its first call, which loads the library."""
+    import copy
+    import pickle
+    un = importlib.import_module(PKG + ".unet")
+    x = torch.zeros(2, 64).half()
+    for m in (qu.AddRMSNorm(nn.RMSNorm(64)), qu.Int8RMSNorm(nn.RMSNorm(64)), qu.Int8LayerNorm(nn.LayerNorm(64)),
+              qu.Int4Linear(64, 16), un.GroupNormNHWC(32, 64)):
+        with contextlib.suppress(RuntimeError):      # the library is loaded, and the CPU refused
+            m(x)
+        assert set(copy.deepcopy(m).state_dict()) == set(m.state_dict())
+        assert type(pickle.loads(pickle.dumps(m))) is type(m)
+        assert all(not isinstance(v, importlib.import_module(PKG + ".csrc._binding")._Base) for v in vars(m).values())
