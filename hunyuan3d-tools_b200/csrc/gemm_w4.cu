@@ -77,7 +77,8 @@ __host__ __device__ constexpr uint32_t make_idesc_f16(bool bf16, uint32_t m, uin
 
 constexpr uint32_t kNegateA = 1u << 13;
 
-// The sum of one output as the definition has it, in order, up to the first NaN.
+// The sum of one output as the definition has it, in order, up to the first NaN.  Rolled up: unrolled it needs 94 registers,
+// 22 more than the kernel, and those leave the next kernel's blocks less room (924 x 1024 -> 2560 10.8 us instead of 10.6).
 template <bool kBf16>
 __device__ __noinline__ float sum_by_definition(const TcArgs& a, int token, int row) {
   const int tiles = a.K >> 6, group = a.K / a.groups, half = row >> 3 & 1, g = row & 7;
@@ -85,14 +86,17 @@ __device__ __noinline__ float sum_by_definition(const TcArgs& a, int token, int 
   const uint16_t* x = a.x + token * a.ldx;
   const uint32_t* w = reinterpret_cast<const uint32_t*>(a.w) + block * tiles * 128 + 16 * g + half;
   float y = 0.0f;
+#pragma unroll 1
   for (int k = 0; k < a.K && y == y; k += 32) {
     const int64_t at = (block * a.groups + k / group) * 16 + 2 * g + half;
     const uint16_t bits = reinterpret_cast<const uint16_t*>(a.scale)[at];
     const float scale = kBf16 ? __uint_as_float(static_cast<uint32_t>(bits) << 16) : __half2float(__ushort_as_half(bits));
     const int zero = a.zero ? a.zero[at] : 8;
     float sum = 0.0f;
+#pragma unroll 1
     for (int t = 0; t < 4; ++t) {      // columns 4t .. 4t + 3 and 16 + 4t .. 16 + 4t + 3
       const uint32_t codes = w[(k >> 6) * 128 + 4 * t + (k >> 4 & 2)];
+#pragma unroll 1
       for (int i = 0; i < 8; ++i) {
         const int code = static_cast<int>(codes >> (4 * (i >> 1) + 16 * (i & 1)) & 15u);
         const uint16_t v = x[k + 4 * t + 16 * (i >> 2) + (i & 3)];
@@ -418,7 +422,7 @@ gemm_w4_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ CUtenso
   }
   // Two numbers a weight cannot give the sum where an activation is infinite: lo is 0 for most weights, and infinity times that
   // is NaN, where infinity times the weight keeps its sign.  A lane's outputs that are NaN are made once more, from the
-  // definition.  (The look for them costs 1 to 2 %: 924 x 1024 -> 2560 10.7 us, without it 10.5.)
+  // definition.  (The look for them costs 0.5 %.)
   if (has_nan<kBf16>(seen)) {
     for (int tok = rank + a.ks * warp; tok < a.tokens && tok0 + tok < a.M; tok += a.ks * static_cast<int>(blockDim.x >> 5)) {
       uint16_t* out = a.out + static_cast<int64_t>(tok0 + tok) * n_out + col;
