@@ -52,7 +52,9 @@ __device__ __forceinline__ void mma_16816(bool bf16, float (&d)[4], uint32_t a0,
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// A nibble c under the exponent of 2^7 (bf16) or 2^10 (fp16) is the number 128 + c or 1024 + c; `minus` is the negative of
+// Integers as the low bits of a number whose exponent is fixed, the usual conversion of packed weights (Y. J. Kim et al., "Who
+// Says Elephants Can't Run", 2022, describe it for these types; the constants follow from the formats):
+// a nibble c under the exponent of 2^7 (bf16) or 2^10 (fp16) is the number 128 + c or 1024 + c; `minus` is the negative of
 // that with the zero point, and the sum is exact.  (As a multiply-add by one: bf16 has no addition of its own.)  fp16 has
 // room for the next nibble where it lies, 1024 + 16 c, and the multiply-add scales it: two shifts in three less.
 template <bool kBf16> constexpr uint32_t kMagic = kBf16 ? 0x43004300u : 0x64006400u;
@@ -100,9 +102,10 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 template <int kPending>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory"); }
 
-// Few tokens (8 at most): bound by the stream of codes and, next to it, by the integer instructions that unpack them (1 x 8192
-// -> 8192 with groups of 128 9.9 us, 3.5 TB/s, with the loop over a stage's tiles rolled up 16; 12 x 1280 -> 640 2.8).  One
-// CTA per SM.  The activations of its tokens lie in shared memory whole; 2^lg_wk warps share a unit of kR blocks of 16
+// Few tokens (8 at most).  1 x 8192 -> 8192 with groups of 128 takes 10.0 us, 3.5 TB/s (with the loop over a stage's tiles rolled
+// up 16), 12 x 1280 -> 640 2.8: neither the stream of codes (5.3 us) nor the instructions that unpack them (72 a tile, 4.7 us on the
+// 128 SMs that a power of two of warps a unit leaves at work; issue slots 56 % used) fill it, but the tiles that a warp has in
+// series, its ring of two stages and the start.  One CTA per SM.  The activations of its tokens lie in shared memory whole; 2^lg_wk warps share a unit of kR blocks of 16
 // rows, each with a range of K, and take `trips` units one after the other without a pause, through rings of their own in
 // shared memory: nothing waits for another warp until the sums are added at the end, in a fixed order.
 // kPlain: no zero points, and scales of the activations' type.
