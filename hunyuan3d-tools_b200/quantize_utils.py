@@ -831,6 +831,9 @@ class Int4Linear(nn.Module):
                 src, cur = state_dict.get(prefix + name), getattr(self, name)
                 if src is None:
                     self.register_buffer(name, None if name != "weight_scale" else cur)
+                elif name == "bias" and tuple(src.shape) != (self.out_features,):
+                    error_msgs.append(f"{prefix}bias: shape {tuple(src.shape)}, expected ({self.out_features},)")
+                    return
                 elif cur is None or cur.shape != src.shape or cur.dtype != src.dtype:
                     dtype = self.weight_scale.dtype if name == "weight_scale" and src.dtype not in half else src.dtype
                     self.register_buffer(name, torch.empty(src.shape, dtype=dtype, device=self.weight_int4.device))

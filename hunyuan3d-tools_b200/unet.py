@@ -204,7 +204,7 @@ class Attention(nn.Module):
 
     def _apply(self, fn, recurse=True):
         super()._apply(fn, recurse)
-        if self.rotary_positions is not None:       # to the module's device, in their own type
+        if type(self.rotary_positions) is dict:       # to the module's device, in their own type
             moved = {n: (t, fn(t)) for n, t in self.rotary_positions.items()}
             self.rotary_positions = {n: v if v.dtype == t.dtype else t.to(v.device) for n, (t, v) in moved.items()}
         return self
@@ -212,9 +212,10 @@ class Attention(nn.Module):
     def _positions_of(self, n):
         if self.rotary_positions is None:
             return None
-        if n not in self.rotary_positions:
-            raise RuntimeError(f"no rotary positions for {n} tokens, only for {sorted(self.rotary_positions)}")
-        return self.rotary_positions[n]
+        try:
+            return self.rotary_positions[n]
+        except KeyError:
+            raise RuntimeError(f"no rotary positions for {n} tokens, only for {sorted(self.rotary_positions)}") from None
 
     def forward(self, x, context=None, kv=None):
         """``kv``: keys and values of the context side by side, where the caller has them already."""

@@ -196,7 +196,8 @@ int hy3d_rotary(const hy3d_rotary_side* sides, int n_sides, int dtype, int64_t b
 /*
  * Linear layer with 4-bit weights, group scales and 16-bit activations:
  *   y[m,n] = epilogue( sum_g scale[n,g] * sum_{k in group g} x[m,k] * (code[n,k] - zero[n,g]) + bias[n] )
- * with fp32 sums of exact products and one rounding to x's type.  x: (M,K) f16 / bf16, row pitch ldx (a multiple of 8).
+ * with fp32 sums of exact products (x up to a fifteenth of fp32's range, 2.2e37) and one rounding to x's type.  x: (M,K) f16 /
+ * bf16, row pitch ldx (a multiple of 8).
  * w: codes 0..15 in tiles of 16 rows x 64 columns, [N/16][K/64][lane][4 words]: lane 4g + t holds rows g and g + 8; words 0
  * and 2 are row g's, words 1 and 3 row g + 8's.  The eight columns of words 0 and 1 are 4t .. 4t+3 and 16 + 4t .. 16 + 4t+3,
  * those of words 2 and 3 32 more; nibble j < 4 of a word is its column 2j, nibble 4 + j its column 2j + 1.

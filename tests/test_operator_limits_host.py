@@ -41,7 +41,7 @@ def test_tensor_memory_is_taken_before_the_next_kernel_may_start(build_mod):
             found += 1
             assert min(starts) > max(takes), f"{name}: the next kernel may start before tensor memory is taken"
             assert "__syncthreads()" in body[max(takes):min(starts)], f"{name}: no barrier behind the allocation"
-    assert found == 5
+    assert found >= 5
 
 
 # ---- angles in 60 digits, apart from the plan ------------------------------------------------
@@ -136,6 +136,8 @@ def test_int4_checkpoints_of_other_shapes_and_types(qu):
                 dict(weight_zero=state["weight_zero"][:, :1]), dict(weight_zero=state["weight_zero"].int())):
         with pytest.raises(RuntimeError, match="weight_scale"):
             qu.Int4Linear(128, 32).load_state_dict({**state, **bad})
+    with pytest.raises(RuntimeError, match="bias"):
+        qu.Int4Linear(128, 32).load_state_dict({**state, "bias": torch.zeros(33)})
     wide = qu.Int4Linear(128, 32)            # scales that were kept in fp32 come back in the layer's type, which the kernels take
     wide.load_state_dict({**state, "weight_scale": state["weight_scale"].float()})
     assert wide.weight_scale.dtype == torch.float16 and torch.equal(wide.dequantize_weight(), layer.dequantize_weight())
